@@ -366,6 +366,91 @@ lm_status lm_moe_route_static(const float* router, const uint16_t* x, int32_t to
                               int32_t experts, int32_t top_k, int32_t norm_topk_prob, float routed_scaling_factor,
                               const float* logit_bias, int32_t* topk_idx, float* topk_w, void* stream);
 
+/*
+ * -- Tokens sorted by expert and back -------------------------------------------
+ * The dispatch and combine that lm_moe_forward does inside, as calls of their own: for a
+ * feed-forward whose expert products the caller runs (lm_mx_matmul), and, with their gradients,
+ * for training one.  No counterpart in the reference, which handles one token at a time
+ * (src/DeepSeekRunner.cpp:273-285).  All pointers are device memory on the current device; calls
+ * are asynchronous on the stream, allocate nothing, and give the same result every time.
+ *
+ * lm_moe_sort_plan gives each of the tokens x top_k pairs its row among the rows sorted by
+ * expert (ties by token, then slot):
+ *   topk_idx  int32 [tokens, top_k], as lm_moe_route writes it; a value outside [0, experts)
+ *             drops the pair (an expert held elsewhere, a padded token)
+ *   offsets   int32 [experts + 1]: expert e's rows are offsets[e] .. offsets[e + 1] - 1
+ *   at        int32 [tokens, top_k]: the pair's row, -1 when dropped
+ * top_k <= LM_SORT_MAX_TOP_K, experts <= 1024, tokens x top_k < 2^31.
+ */
+#define LM_SORT_MAX_TOP_K 64
+lm_status lm_moe_sort_plan(const int32_t* topk_idx, int64_t tokens, int32_t top_k, int32_t experts, int32_t* offsets,
+                           int32_t* at, void* stream);
+/* rows[at[t, j]] = x[t] for every pair with 0 <= at < n_rows; other rows are left as they were.
+ * `at` here and below is a plan's: no row stands in it twice.
+ * Rows are plain bytes (row_bytes of them, strides in bytes), so values of any type, MX codes and
+ * MX scales sort alike.  x and rows must not overlap. */
+lm_status lm_moe_sort_rows(const void* x, int64_t x_stride, const int32_t* at, int64_t tokens, int32_t top_k,
+                           int64_t row_bytes, void* rows, int64_t rows_stride, int64_t n_rows, void* stream);
+/* y[t] = sum over j of weights[t, j] * rows[at[t, j]] (weights NULL: 1), f32 sums in slot order,
+ * rounded once; a token without rows gets 0.  accumulate != 0 adds to y (before the rounding).
+ * rows [n_rows, cols] of `dtype` (LM_DTYPE_F32, _BF16 or _F16); y [tokens, cols] of the same type
+ * or f32.  Without weights this is also the gradient of lm_moe_sort_rows. */
+lm_status lm_moe_unsort_rows(const void* rows, int32_t dtype, int64_t n_rows, const int32_t* at, const float* weights,
+                             int64_t tokens, int32_t top_k, int64_t cols, void* y, int32_t y_dtype, int32_t accumulate,
+                             void* stream);
+/* The gradient of lm_moe_unsort_rows with weights:
+ *   grad_rows[at[t, j]] = weights[t, j] * grad_y[t]     (other rows are left as they were)
+ *   grad_weights[t, j]  = <grad_y[t], rows[at[t, j]]>   (f32; 0 when dropped)
+ * grad_y, rows and grad_rows of one type.  grad_rows may be rows itself, not overlap it otherwise. */
+lm_status lm_moe_unsort_rows_backward(const void* grad_y, const void* rows, int32_t dtype, int64_t n_rows,
+                                      const int32_t* at, const float* weights, int64_t tokens, int32_t top_k,
+                                      int64_t cols, void* grad_rows, float* grad_weights, void* stream);
+
+/*
+ * -- Microscaled (MX) matrices ----------------------------------------------------
+ * Rows of 4-bit (E2M1) or 8-bit (E4M3) floating point with one power-of-two scale (E8M0) for each
+ * 32 columns, as the OCP microscaling formats define them: weights in a quarter of their bf16
+ * bytes, activations in half.  A matrix [rows, cols] is two device arrays:
+ *   data    [rows, lm_mx_data_pitch]   E2M1: two codes a byte, the even column in the low half;
+ *                                      E4M3: a byte a code; zero codes up to a multiple of 128 columns
+ *   scales  [rows, lm_mx_scale_pitch]  scale 2^(byte - 127); zero bytes up to a multiple of 16
+ * data starts on a 32-byte boundary, scales on a 16-byte one.  The padding has to hold zeros, as
+ * lm_mx_quantize writes it.  rows <= LM_MX_MAX_ROWS, cols <= LM_MX_MAX_COLS.  The calls
+ * without a context allocate nothing; they run on the current device and the given stream.
+ */
+#define LM_MX_E2M1 1
+#define LM_MX_E4M3 2
+#define LM_MX_MAX_ROWS 2147483647
+#define LM_MX_MAX_COLS 16777216
+#define LM_MX_MAX_GROUPS 1024
+/* Bytes of one row of data / of scales (0 for a bad format or size).  Host only. */
+int64_t lm_mx_data_pitch(int32_t format, int64_t cols);
+int64_t lm_mx_scale_pitch(int64_t cols);
+/* values [rows, cols] of `dtype` (LM_DTYPE_F32, _BF16 or _F16), row_stride elements apart, to MX.
+ * A block's scale byte is the biased f32 exponent of its largest magnitude less 2 (E2M1) or 8
+ * (E4M3), at least 0; codes are rounded to nearest even and clamped to +-6 or +-448.  A block with
+ * a NaN or an infinity gets scale byte 255 (NaN) and zero codes. */
+lm_status lm_mx_quantize(const void* values, int32_t dtype, int64_t rows, int64_t cols, int64_t row_stride, int32_t format,
+                         uint8_t* data, uint8_t* scales, void* stream);
+/* The values that an MX matrix stands for, rounded to `dtype`. */
+lm_status lm_mx_dequantize(const uint8_t* data, const uint8_t* scales, int32_t format, int64_t rows, int64_t cols,
+                           void* values, int32_t dtype, int64_t row_stride, void* stream);
+/*
+ * Grouped product of MX matrices: out[r, :] = W_g x[r, :] for the rows r of group g, f32 sums
+ * rounded once to out_dtype (LM_DTYPE_F32, _BF16 or _F16).
+ *   x, x_scales  [rows, k] in x_format (E4M3 or E2M1), sorted by group
+ *   w, w_scales  [groups, n, k] in E2M1
+ *   offsets      device int32 [groups + 1]: group g's rows are offsets[g] .. offsets[g + 1] - 1
+ *                (lm_moe_sort_plan's); NULL with groups = 1: all rows.  Values are clamped to
+ *                [0, rows] and to ascending order; rows of no group are left as they were
+ *   out          [rows, n], out_stride elements apart
+ * k >= 1, groups <= LM_MX_MAX_GROUPS, groups * n < 2^31.  A NaN or infinity affects only its own row (x)
+ * or its group's column (w).
+ */
+lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_format, int64_t rows, const uint8_t* w,
+                       const uint8_t* w_scales, int32_t groups, int64_t n, int64_t k, const int32_t* offsets, void* out,
+                       int32_t out_dtype, int64_t out_stride, void* stream);
+
 /* ── gemm:: kernels on device memory (include/Gemm.hpp:23-72) ──────────────── */
 
 /* gemm::kernel_description (src/Gemm.cpp:108-123): which kernels this build runs, for
@@ -389,6 +474,16 @@ lm_status lm_gemm_silu_multiply(const float* gate, const float* up, float* desti
 /* gemm::rms_norm (src/Gemm.cpp:197-207), in place over each of `rows` rows. */
 lm_status lm_gemm_rms_norm(float* values, const float* weight, int64_t rows, int64_t count,
                            float epsilon, void* stream);
+/* The residual's addition and gemm::rms_norm in one pass, with an MX output for lm_mx_matmul:
+ *   sum  = hidden + delta                           (rounded to hidden's type; delta NULL: hidden)
+ *   norm = sum * rsqrt(mean(sum^2) + epsilon) * weight
+ * and norm, in f32, goes to an MX matrix [rows, count] (data, scales, format as above) and, with
+ * out_bf16 not NULL, to bf16 [rows, count] (what lm_moe_route reads).  hidden and delta are f32 or
+ * bf16 (LM_DTYPE_*), all rows contiguous; sum has hidden's type and may be hidden itself or delta
+ * when their types agree.  The squares are summed in f64. */
+lm_status lm_gemm_add_rms_norm_mx(const void* hidden, int32_t dtype, const void* delta, int32_t delta_dtype,
+                                  const float* weight, int64_t rows, int64_t count, float epsilon, void* sum,
+                                  uint16_t* out_bf16, int32_t format, uint8_t* data, uint8_t* scales, void* stream);
 /* gemm::axpy (src/Gemm.cpp:191-195): destination += scale * source. */
 lm_status lm_gemm_axpy(float scale, const float* source, float* destination, int64_t count,
                        void* stream);

@@ -28,6 +28,8 @@ PROFILE_SLOT_NAMES = ["gather_rows", "route", "router_topk", "dispatch_scan", "p
 LM_DTYPE_UNKNOWN, LM_DTYPE_BF16, LM_DTYPE_F16, LM_DTYPE_F32, LM_DTYPE_OTHER = 0, 1, 2, 3, 4
 LM_SAFETENSORS_MAX_DIMS = 8
 
+LM_MX_E2M1, LM_MX_E4M3 = 1, 2
+
 LM_TOPK_GREEDY = 0
 LM_TOPK_GROUP_LIMITED_GREEDY = 1
 LM_DEBUG_GRID_EXTRA = 1
@@ -92,6 +94,16 @@ SIGNATURES = {
     "lm_moe_profile_trace": (_i32, [_vp, _vp, _i32, _vp]),
     "lm_moe_profile_ep_timeline": (_i32, [_vp, _vp, _i32, C.POINTER(C.c_int32)]),
     "lm_moe_route_static": (_i32, [_vp, _vp, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp]),
+    "lm_moe_sort_plan": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp, _vp]),
+    "lm_moe_sort_rows": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _vp, _i64, _i64, _vp]),
+    "lm_moe_unsort_rows": (_i32, [_vp, _i32, _i64, _vp, _vp, _i64, _i32, _i64, _vp, _i32, _i32, _vp]),
+    "lm_moe_unsort_rows_backward": (_i32, [_vp, _vp, _i32, _i64, _vp, _vp, _i64, _i32, _i64, _vp, _vp, _vp]),
+    "lm_mx_data_pitch": (_i64, [_i32, _i64]),
+    "lm_mx_scale_pitch": (_i64, [_i64]),
+    "lm_mx_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp, _vp]),
+    "lm_mx_dequantize": (_i32, [_vp, _vp, _i32, _i64, _i64, _vp, _i32, _i64, _vp]),
+    "lm_mx_matmul": (_i32, [_vp, _vp, _i32, _i64, _vp, _vp, _i32, _i64, _i64, _vp, _vp, _i32, _i64, _vp]),
+    "lm_gemm_add_rms_norm_mx": (_i32, [_vp, _i32, _vp, _i32, _vp, _i64, _i64, _f32, _vp, _vp, _i32, _vp, _vp, _vp]),
     "lm_kernel_description": (C.c_char_p, []),
     "lm_gemm_matvec_bf16": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp]),
     "lm_gemm_matvec_bf16_accumulate": (_i32, [_vp, _vp, _vp, _i64, _i64, _f32, _vp]),

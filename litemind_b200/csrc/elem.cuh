@@ -1,0 +1,95 @@
+// elem.cuh -- f32, bf16 and f16 elements behind an LM_DTYPE_* constant, and what the entry points
+// over them share: argument checks and the choice of an instantiation.
+#pragma once
+
+#include <cstdint>
+#include <cstring>
+#include <type_traits>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "litemind_moe.h"
+
+namespace lm {
+
+// ── element types ─────────────────────────────────────────────────────────
+template <int DT>
+struct Elem;
+template <>
+struct Elem<LM_DTYPE_F32> {
+    using T = float;
+    static __device__ __forceinline__ float widen(float v) { return v; }
+    static __device__ __forceinline__ float narrow(float v) { return v; }
+};
+template <>
+struct Elem<LM_DTYPE_BF16> {
+    using T = __nv_bfloat16;
+    static __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+    static __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
+};
+template <>
+struct Elem<LM_DTYPE_F16> {
+    using T = __half;
+    static __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+    static __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
+};
+
+// Eight consecutive elements from / to a 16-byte aligned address.
+template <int DT>
+__device__ __forceinline__ void load8(const typename Elem<DT>::T* p, float (&v)[8]) {
+    if constexpr (DT == LM_DTYPE_F32) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+        const uint4 q = *reinterpret_cast<const uint4*>(p);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            typename Elem<DT>::T e[2];
+            memcpy(e, &w[i], 4);
+            v[2 * i] = Elem<DT>::widen(e[0]);
+            v[2 * i + 1] = Elem<DT>::widen(e[1]);
+        }
+    }
+}
+template <int DT>
+__device__ __forceinline__ void store8(typename Elem<DT>::T* p, const float (&v)[8]) {
+    if constexpr (DT == LM_DTYPE_F32) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const typename Elem<DT>::T e[2] = {Elem<DT>::narrow(v[2 * i]), Elem<DT>::narrow(v[2 * i + 1])};
+            memcpy(&w[i], e, 4);
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// ── entry points ─────────────────────────────────────────────────────────
+inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+inline int64_t elem_size(int32_t dtype) { return dtype == LM_DTYPE_F32 ? 4 : 2; }
+inline bool is_float_type(int32_t dtype) { return dtype == LM_DTYPE_F32 || dtype == LM_DTYPE_BF16 || dtype == LM_DTYPE_F16; }
+
+// Each calls f with the choice as a compile-time constant.
+template <class F>
+void with_dtype(int32_t dtype, F&& f) {
+    if (dtype == LM_DTYPE_F32) f(std::integral_constant<int, LM_DTYPE_F32>{});
+    else if (dtype == LM_DTYPE_BF16) f(std::integral_constant<int, LM_DTYPE_BF16>{});
+    else f(std::integral_constant<int, LM_DTYPE_F16>{});
+}
+template <class F>
+void with_format(int32_t format, F&& f) {
+    if (format == LM_MX_E2M1) f(std::integral_constant<int, LM_MX_E2M1>{});
+    else f(std::integral_constant<int, LM_MX_E4M3>{});
+}
+template <class F>
+void with_bool(bool b, F&& f) {
+    if (b) f(std::true_type{});
+    else f(std::false_type{});
+}
+
+}  // namespace lm

@@ -280,6 +280,9 @@ cudaError_t launch_add_rows(float* dst, const float* src, int64_t count, cudaStr
 cudaError_t launch_pack_swiglu(const uint16_t* gate, const uint16_t* up, const uint16_t* down, int inter, int hidden,
                                uint16_t* w13, uint16_t* w2, int sms, cudaStream_t stream);
 const std::string& context_free_error();
+// The same message for an entry point without a context: a refused argument, or a launch's status.
+lm_status context_free_fail(lm_status status, const char* message);
+lm_status context_free_finish(cudaError_t e);
 
 // Raises `kernel`'s dynamic shared-memory limit to `bytes` on the current device.
 // The attribute belongs to the device's context, so it is set once per device
