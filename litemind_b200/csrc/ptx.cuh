@@ -289,6 +289,40 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
+// ── block-scaled MMA: 8- and 4-bit operands with E8M0 scales of 32 columns ──
+// D[tmem] (+)= (A * 2^sa) * (B * 2^sb)^T over 32 columns (kind::mxf8f6f4).  A 4-bit operand sits in
+// shared memory as TMA's 16U4_ALIGN16B type writes it: 16 codes in 8 bytes, then 8 unused bytes, so
+// that 128 columns fill the same 128-byte swizzled row as 8-bit codes do.  Scales sit in TMEM: word
+// (lane i, column c) of `sfa` holds four scale bytes of row 32 c + i, the same in each 32-lane
+// quadrant; the descriptor names the byte.
+__device__ __forceinline__ void umma_mx(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa,
+                                        uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+constexpr uint32_t kUmmaE4M3 = 0, kUmmaE2M1 = 5;  // operand formats
+__host__ __device__ constexpr uint32_t umma_idesc_mx(uint32_t a_format, uint32_t b_format, int M, int N, int scale_byte) {
+    return (static_cast<uint32_t>(scale_byte) << 4)     // B's scale byte
+           | (a_format << 7) | (b_format << 10)
+           | (static_cast<uint32_t>(N >> 3) << 17)      // N / 8
+           | (1u << 23)                                 // scales are E8M0
+           | (static_cast<uint32_t>(M >> 4) << 24)      // M / 16
+           | (static_cast<uint32_t>(scale_byte) << 29); // A's scale byte
+}
+// 32 lanes x 32 bits, 16 consecutive columns per thread; tmem_st_wait before the fence that publishes them.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
 // ── CTA pairs (clusters of 2) ─────────────────────────────────────────────
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;
