@@ -305,5 +305,7 @@ bool encode_tensor_map_bf16(CUtensorMap* map, const void* base, uint64_t rows, u
                             uint32_t box_rows, uint32_t box_cols, std::string& error);
 bool encode_tensor_map_mx(CUtensorMap* map, const void* base, bool four_bit, uint64_t rows, uint64_t cols, uint32_t box_rows,
                           std::string& error);
+bool encode_tensor_map_mx_scales(CUtensorMap* map, const void* base, uint64_t rows, uint64_t pitch, uint32_t box_rows,
+                                 uint32_t box_cols, std::string& error);
 
 }  // namespace lm

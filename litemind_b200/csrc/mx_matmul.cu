@@ -5,12 +5,15 @@
 //
 // The weights are the MMA's M side, so that a few rows of X cost a narrow N instead of a padded M.
 // One persistent CTA an SM walks the tiles (group, BN rows of X, 128 rows of W).  Its warps:
-//   0      TMA producer: a ring of stages of 128 columns.  4-bit codes travel packed (half a byte a
+//   0      TMA producer: a ring of stages of 256 columns.  4-bit codes travel packed (half a byte a
 //          column from HBM and L2) and are spread by the TMA into the MMA's padded form.
-//   1      MMA issuer: four block-scaled MMAs of 32 columns a stage, one scale byte each
-//   4-7    scales, straight from their rows to TMEM (no shared memory): a lane loads 16 bytes of a
-//          row, the scales of four stages; each warp writes its own quadrant's copy
+//   1      MMA issuer: eight block-scaled MMAs of 32 columns a stage
+//   2      scale producer: 32 bytes of each row, the scales of 1024 columns, to shared memory by TMA,
+//          up to three such chunks ahead
+//   4-7    scales from shared memory to TMEM, each warp to its own quadrant
 //   8-11   epilogue: TMEM to registers to out, rounded once; double buffered against the MMA
+// A stage costs the issuer about 400 cycles of waits, descriptors and commits whatever its width,
+// and four MMAs take 200 (N = 16) to 256 (N = 128): hence eight of them a stage.
 // Every wait is bounded (ptx.cuh): a pipeline that stalls records a status for lm_mx_sync.
 #include "moe_internal.h"
 #include "mx_block.cuh"
@@ -22,37 +25,35 @@ namespace lm {
 namespace {
 
 constexpr int kBlockM = 128;
-constexpr int kStageCols = 128;     // columns of a stage: one 128-byte row of the swizzled tiles
-constexpr int kSfStages = 4;        // stages of one scale group: 16 scale bytes a row
+constexpr int kBoxCols = 128;       // columns of a TMA box: one 128-byte row of the swizzled tiles
+constexpr int kStageBoxes = 2;
+constexpr int kChunkBoxes = 8;      // a chunk of scales: 32 bytes a row
+constexpr int kChunkBytes = 32;
+constexpr int kChunks = 3;
 constexpr int kThreads = 384;
 constexpr int kSms = 148;
-constexpr int kATileBytes = kBlockM * kStageCols;
+constexpr int kABoxBytes = kBlockM * kBoxCols;
 
 template <int BN>
 struct Cfg {
-    static constexpr int kBTileBytes = BN * kStageCols;
-    static constexpr int kStageBytes = kATileBytes + kBTileBytes;
-    static constexpr int kFit = 212 * 1024 / kStageBytes;
-    static constexpr int kStages = kFit > 12 ? 12 : kFit;
-    static constexpr int kSmemBytes = 1024 + kStages * kStageBytes;
-    static constexpr int kAccs = BN <= 128 ? 2 : 1;                // accumulators in TMEM
-    static constexpr int kSfbCols = BN <= 128 ? 4 : BN / 32;       // TMEM columns of a stage's X scales
-    static constexpr int kSfCols = kSfStages * (4 + kSfbCols);     // TMEM columns of a scale group
-    static constexpr int kSfGroups = std::min(8, (512 - kAccs * BN) / kSfCols);
-    static_assert(BN % 16 == 0 && BN >= 16 && BN <= 256, "N of an M = 128 MMA");
+    static constexpr int kBBoxBytes = BN * kBoxCols;
+    static constexpr int kStageBytes = kStageBoxes * (kABoxBytes + kBBoxBytes);
+    static constexpr int kScaleBytes = (kBlockM + BN) * kChunkBytes;
+    static constexpr int kFit = (216 * 1024 - kChunks * kScaleBytes) / kStageBytes;
+    static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kChunks * kScaleBytes;
+    static constexpr int kSfCols = kChunkBoxes * (4 + 4);  // TMEM columns of a chunk: per box 4 of W's scales, 4 of X's
+    static constexpr int kSfGroups = (512 - 2 * BN) / kSfCols;
+    static_assert(BN % 16 == 0 && BN >= 16 && BN <= 128, "N of an M = 128 MMA, two accumulators");
     static_assert(kStages >= 3 && kSfGroups >= 2, "rings");
 };
 
 struct Args {
-    const uint8_t* x_scales;
-    const uint8_t* w_scales;
     const int32_t* offsets;  // or null: one group of all rows
     void* out;
     int64_t out_stride;
-    int64_t scale_pitch;
-    int64_t w_rows;  // groups * n
     int rows, groups, n;
-    int k_stages;
+    int k_boxes;
     int x_four_bit;
     int out_dtype;
     int* status;
@@ -130,25 +131,30 @@ __device__ __forceinline__ void store_columns(void* out, int64_t at, int64_t str
 
 template <int BN>
 __global__ void __launch_bounds__(kThreads, 1)
-    mx_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Args a) {
+    mx_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                     const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_xs, const Args a) {
     using C = Cfg<BN>;
     constexpr int S = C::kStages, G = C::kSfGroups;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ int s_cut[LM_MX_MAX_GROUPS + 1], s_tiles[LM_MX_MAX_GROUPS + 1];
-    __shared__ uint64_t full[S], empty[S], sf_full[G], sf_empty[G], tmem_full[C::kAccs], tmem_empty[C::kAccs], drain;
+    __shared__ uint64_t full[S], empty[S], chunk_full[kChunks], chunk_empty[kChunks], sf_full[G], sf_empty[G], tmem_full[2], tmem_empty[2], drain;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     uint8_t* smem_a = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* smem_b = smem_a + S * kATileBytes;
+    uint8_t* smem_b = smem_a + S * kStageBoxes * kABoxBytes;
+    uint8_t* smem_s = smem_b + S * kStageBoxes * C::kBBoxBytes;  // chunks: 128 rows of W's scales, then BN of X's
     volatile int* abort_flag = &s_abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (warp == 0 && lane == 0) {
         tma_prefetch_desc(&map_w);
         tma_prefetch_desc(&map_x);
+        tma_prefetch_desc(&map_ws);
+        tma_prefetch_desc(&map_xs);
         for (int i = 0; i < S; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+        for (int i = 0; i < kChunks; ++i) mbar_init(&chunk_full[i], 1), mbar_init(&chunk_empty[i], 4);
         for (int i = 0; i < G; ++i) mbar_init(&sf_full[i], 4), mbar_init(&sf_empty[i], 1);
-        for (int i = 0; i < C::kAccs; ++i) mbar_init(&tmem_full[i], 1), mbar_init(&tmem_empty[i], 4);
+        for (int i = 0; i < 2; ++i) mbar_init(&tmem_full[i], 1), mbar_init(&tmem_empty[i], 4);
         mbar_init(&drain, 1);
         s_abort = 0;
         fence_mbar_init();
@@ -162,134 +168,151 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    const uint32_t tmem_sf = tmem + C::kAccs * BN;
+    const uint32_t tmem_sf = tmem + 2 * BN;
     const int m_blocks = (a.n + kBlockM - 1) / kBlockM;
     const int total = s_tiles[a.groups] * m_blocks;
 
+    // In the issuing warps all lanes walk the loop and an elected one issues, so that descriptors and
+    // addresses stay in uniform registers (under `if (lane == 0)` a stage took twice as long).
     if (warp == 0) {
-        if (lane == 0) {
-            const uint32_t bytes = kATileBytes / 2 + (a.x_four_bit ? C::kBTileBytes / 2 : C::kBTileBytes);
-            int stage = 0;
-            uint32_t phase = 0, issued = 0, issued_phase = 0;
-            bool ok = true;
-            for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
-                const Tile tile = tile_at<BN>(a, s_cut, s_tiles, t, m_blocks);
-                const int w_row = tile.group * a.n + tile.n0;
-                for (int s = 0; s < a.k_stages; ++s) {
-                    if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, a.status, kDevTimeoutProducer)) {
-                        ok = false;
-                        break;
-                    }
-                    mbar_arrive_expect_tx(&full[stage], bytes);
-                    tma_load_2d(smem_a + stage * kATileBytes, &map_w, &full[stage], s * kStageCols, w_row);
-                    tma_load_2d(smem_b + stage * C::kBTileBytes, &map_x, &full[stage], s * kStageCols, tile.row0);
-                    issued |= 1u << stage;
-                    issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
-                    if (++stage == S) stage = 0, phase ^= 1u;
-                }
-            }
-            if (!ok)  // copies in flight land before the CTA's shared memory is given up
-                for (int i = 0; i < S; ++i)
-                    if (issued & (1u << i)) mbar_wait_drain(&full[i], (issued_phase >> i) & 1u, 100000000ull);
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
-            int stage = 0, sg = 0, acc = 0;
-            uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
-            bool ok = true, any = false;
-            const uint32_t b_format = a.x_four_bit ? kUmmaE2M1 : kUmmaE4M3;
-            for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
-                if (!mbar_wait(&tmem_empty[acc], acc_phase ^ 1u, abort_flag, a.status, kDevTimeoutMma)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t d = tmem + acc * BN;
-                for (int s = 0; s < a.k_stages; ++s) {
-                    const int sub = s & (kSfStages - 1);
-                    if (sub == 0 && !mbar_wait(&sf_full[sg], sf_phase, abort_flag, a.status, kDevTimeoutMma)) {
-                        ok = false;
-                        break;
-                    }
-                    if (!mbar_wait(&full[stage], phase, abort_flag, a.status, kDevTimeoutMma)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint64_t da = umma_desc_sw128(smem_u32(smem_a + stage * kATileBytes));
-                    const uint64_t db = umma_desc_sw128(smem_u32(smem_b + stage * C::kBTileBytes));
-                    const uint32_t sfa = tmem_sf + sg * C::kSfCols + sub * 4;
-                    const uint32_t sfb = tmem_sf + sg * C::kSfCols + 4 * kSfStages + sub * C::kSfbCols;
-#pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)  // 32 columns are 32 bytes, 2 in the descriptor's units
-                        umma_mx(d, da + 2 * kk, db + 2 * kk, umma_idesc_mx(kUmmaE2M1, b_format, kBlockM, BN, kk), sfa, sfb,
-                                s != 0 || kk != 0);
-                    any = true;
-                    umma_commit(&empty[stage]);
-                    if (++stage == S) stage = 0, phase ^= 1u;
-                    if (sub == kSfStages - 1 || s == a.k_stages - 1) {
-                        umma_commit(&sf_empty[sg]);
-                        if (++sg == G) sg = 0, sf_phase ^= 1u;
-                    }
-                }
-                if (!ok) break;
-                umma_commit(&tmem_full[acc]);
-                if (++acc == C::kAccs) acc = 0, acc_phase ^= 1u;
-            }
-            if (!ok && any) {  // the MMAs issued so far end before TMEM is released
-                umma_commit(&drain);
-                mbar_wait_drain(&drain, 0, 100000000ull);
-            }
-        }
-    } else if (warp >= 4 && warp < 8) {
-        const uint32_t quad = static_cast<uint32_t>(warp & 3) * 32u << 16;
-        constexpr int kXRows = (BN + 31) / 32;
-        const int sf_groups = (a.k_stages + kSfStages - 1) / kSfStages;
-        int sg = 0;
-        uint32_t phase = 0;
+        const uint32_t box_bytes = kABoxBytes / 2 + (a.x_four_bit ? C::kBBoxBytes / 2 : C::kBBoxBytes);
+        int stage = 0;
+        uint32_t phase = 0, issued = 0, issued_phase = 0;
         bool ok = true;
         for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
             const Tile tile = tile_at<BN>(a, s_cut, s_tiles, t, m_blocks);
-            const int64_t w_row = static_cast<int64_t>(tile.group) * a.n + tile.n0 + lane;
-            const uint8_t* wp = a.w_scales + w_row * a.scale_pitch;
-            const uint8_t* xp = a.x_scales + (static_cast<int64_t>(tile.row0) + lane) * a.scale_pitch;
-            for (int q = 0; ok && q < sf_groups; ++q) {
-                uint4 w[4], x[kXRows];
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    w[c] = w_row + 32 * c < a.w_rows ? __ldg(reinterpret_cast<const uint4*>(wp + 32 * c * a.scale_pitch + 16 * q))
-                                                     : make_uint4(0, 0, 0, 0);
-#pragma unroll
-                for (int c = 0; c < kXRows; ++c)
-                    x[c] = tile.row0 + lane + 32 * c < a.rows ? __ldg(reinterpret_cast<const uint4*>(xp + 32 * c * a.scale_pitch + 16 * q))
-                                                              : make_uint4(0, 0, 0, 0);
-                // lane 0 polls: the warp goes on together
-                int go = 1;
-                if (lane == 0) go = mbar_wait(&sf_empty[sg], phase ^ 1u, abort_flag, a.status, kDevTimeoutProducer);
-                ok = __shfl_sync(0xffffffffu, go, 0) != 0;
+            const int w_row = tile.group * a.n + tile.n0;
+            for (int b = 0; b < a.k_boxes; b += kStageBoxes) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, abort_flag, a.status, kDevTimeoutProducer));
+                if (!ok) break;
+                if (elect_one()) {
+                    const int boxes = min(kStageBoxes, a.k_boxes - b);
+                    mbar_arrive_expect_tx(&full[stage], boxes * box_bytes);
+                    for (int i = 0; i < boxes; ++i) {
+                        tma_load_2d(smem_a + (stage * kStageBoxes + i) * kABoxBytes, &map_w, &full[stage], (b + i) * kBoxCols, w_row);
+                        tma_load_2d(smem_b + (stage * kStageBoxes + i) * C::kBBoxBytes, &map_x, &full[stage], (b + i) * kBoxCols, tile.row0);
+                    }
+                }
+                __syncwarp();
+                issued |= 1u << stage;
+                issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+                if (++stage == S) stage = 0, phase ^= 1u;
+            }
+        }
+        if (!ok)  // copies in flight land before the CTA's shared memory is given up
+            for (int i = 0; i < S; ++i)
+                if (issued & (1u << i)) mbar_wait_drain(&full[i], (issued_phase >> i) & 1u, 100000000ull);
+    } else if (warp == 1) {
+        int stage = 0, sg = 0, acc = 0;
+        uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
+        bool ok = true, any = false, seen = false;
+        const uint32_t format = (a.x_four_bit ? kUmmaE2M1 : kUmmaE4M3) << 10;
+        const uint64_t desc_a = umma_desc_sw128(smem_u32(smem_a)), desc_b = umma_desc_sw128(smem_u32(smem_b));
+        for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&tmem_empty[acc], acc_phase ^ 1u, abort_flag, a.status, kDevTimeoutMma));
+            const uint32_t d = tmem + acc * BN;
+            for (int b = 0; ok && b < a.k_boxes; b += kStageBoxes) {
+                if (b % kChunkBoxes == 0) ok = mbar_wait(&sf_full[sg], sf_phase, abort_flag, a.status, kDevTimeoutMma);
+                if (!seen) ok = ok && mbar_wait(&full[stage], phase, abort_flag, a.status, kDevTimeoutMma);
+                if (b % kChunkBoxes == 0 || !seen) ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t at = tmem_sf + quad + sg * C::kSfCols;
-                uint32_t r[16];
+                const int next = stage + 1 == S ? 0 : stage + 1;
+                // A look at the next stage while the tensor cores still work: even the wait for a
+                // complete barrier costs as much as an MMA.
+                const bool look = mbar_test(&full[next], phase ^ (next == 0));
+                const bool last = b + kStageBoxes >= a.k_boxes;
+                const bool sf_end = last || (b + kStageBoxes) % kChunkBoxes == 0;
+                if (elect_one()) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) r[c] = w[c].x, r[4 + c] = w[c].y, r[8 + c] = w[c].z, r[12 + c] = w[c].w;
-                tmem_st16(at, r);
+                    for (int i = 0; i < kStageBoxes; ++i) {
+                        if (b + i < a.k_boxes) {
+                            const uint64_t da = desc_a + static_cast<uint32_t>((stage * kStageBoxes + i) * (kABoxBytes >> 4));
+                            const uint64_t db = desc_b + static_cast<uint32_t>((stage * kStageBoxes + i) * (C::kBBoxBytes >> 4));
+                            const uint32_t sf = tmem_sf + sg * C::kSfCols + (b % kChunkBoxes + i) * 8;
 #pragma unroll
-                for (int h = 0; h < C::kSfbCols / 4; ++h) {  // 16 words: X rows in fours, or two stages of eight
-                    uint32_t u[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int word = h * 16 + i, sub = word / C::kSfbCols, c = word % C::kSfbCols;
-                        u[i] = 0;
-                        if (c < kXRows) u[i] = sub == 0 ? x[c].x : sub == 1 ? x[c].y : sub == 2 ? x[c].z : x[c].w;
+                            for (int kk = 0; kk < 4; ++kk)  // 32 columns are 32 bytes, 2 in the descriptor's units
+                                umma_mx(d, da + 2 * kk, db + 2 * kk, umma_idesc_mx(kUmmaE2M1, 0, kBlockM, BN, kk) | format, sf, sf + 4,
+                                        b != 0 || i != 0 || kk != 0);
+                        }
                     }
-                    tmem_st16(at + 16 + 16 * h, u);
+                    umma_commit(&empty[stage]);
+                    if (sf_end) umma_commit(&sf_empty[sg]);
+                    if (last) umma_commit(&tmem_full[acc]);
+                }
+                __syncwarp();
+                any = true;
+                seen = __all_sync(0xffffffffu, look);
+                phase ^= next == 0, stage = next;
+                if (sf_end && ++sg == G) sg = 0, sf_phase ^= 1u;
+            }
+            if (++acc == 2) acc = 0, acc_phase ^= 1u;
+        }
+        if (!ok && any) {  // the MMAs issued so far end before TMEM is released
+            if (elect_one()) umma_commit(&drain);
+            __syncwarp();
+            mbar_wait_drain(&drain, 0, 100000000ull);
+        }
+    } else if (warp == 2) {
+        int chunk = 0;
+        uint32_t phase = 0, issued = 0, issued_phase = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
+            const Tile tile = tile_at<BN>(a, s_cut, s_tiles, t, m_blocks);
+            for (int b = 0; b < a.k_boxes; b += kChunkBoxes) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&chunk_empty[chunk], phase ^ 1u, abort_flag, a.status, kDevTimeoutProducer));
+                if (!ok) break;
+                if (elect_one()) {
+                    uint8_t* dst = smem_s + chunk * C::kScaleBytes;
+                    mbar_arrive_expect_tx(&chunk_full[chunk], C::kScaleBytes);
+                    tma_load_2d(dst, &map_ws, &chunk_full[chunk], b / kChunkBoxes * kChunkBytes, tile.group * a.n + tile.n0);
+                    tma_load_2d(dst + kBlockM * kChunkBytes, &map_xs, &chunk_full[chunk], b / kChunkBoxes * kChunkBytes, tile.row0);
+                }
+                __syncwarp();
+                issued |= 1u << chunk;
+                issued_phase = (issued_phase & ~(1u << chunk)) | (phase << chunk);
+                if (++chunk == kChunks) chunk = 0, phase ^= 1u;
+            }
+        }
+        if (!ok)
+            for (int i = 0; i < kChunks; ++i)
+                if (issued & (1u << i)) mbar_wait_drain(&chunk_full[i], (issued_phase >> i) & 1u, 100000000ull);
+    } else if (warp >= 4 && warp < 8) {
+        const uint32_t quad = static_cast<uint32_t>(warp & 3) * 32u << 16;
+        constexpr int kXRows = (BN + 31) / 32;
+        int sg = 0, chunk = 0;
+        uint32_t phase = 0, chunk_phase = 0;
+        bool ok = true;
+        for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
+            for (int b = 0; ok && b < a.k_boxes; b += kChunkBoxes) {
+                // Every lane waits for what it reads; a lane that gave up takes its warp along.
+                ok = mbar_wait(&chunk_full[chunk], chunk_phase, abort_flag, a.status, kDevTimeoutProducer);
+                ok = ok && mbar_wait(&sf_empty[sg], phase ^ 1u, abort_flag, a.status, kDevTimeoutProducer);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const uint8_t* src = smem_s + chunk * C::kScaleBytes + lane * kChunkBytes;
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {  // 8 bytes of a row are the scales of two boxes: 16 columns of TMEM
+                    uint32_t r[16];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const uint2 w = *reinterpret_cast<const uint2*>(src + 32 * c * kChunkBytes + 8 * h);
+                        uint2 x = make_uint2(0u, 0u);
+                        if (c < kXRows && (BN >= 32 || lane < BN)) x = *reinterpret_cast<const uint2*>(src + (kBlockM + 32 * c) * kChunkBytes + 8 * h);
+                        r[c] = w.x, r[8 + c] = w.y, r[4 + c] = x.x, r[12 + c] = x.y;
+                    }
+                    tmem_st16(tmem_sf + quad + sg * C::kSfCols + 16 * h, r);
                 }
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sf_full[sg]);
+                if (lane == 0) {
+                    mbar_arrive(&sf_full[sg]);
+                    mbar_arrive(&chunk_empty[chunk]);
+                }
                 if (++sg == G) sg = 0, phase ^= 1u;
+                if (++chunk == kChunks) chunk = 0, chunk_phase ^= 1u;
             }
         }
     } else if (warp >= 8) {
@@ -320,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&tmem_empty[acc]);
-            if (++acc == C::kAccs) acc = 0, acc_phase ^= 1u;
+            if (++acc == 2) acc = 0, acc_phase ^= 1u;
         }
     }
     tc_fence_before();
@@ -329,16 +352,28 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 1) tmem_dealloc(tmem, 512);
 }
 
+struct Matrix {
+    const uint8_t* codes;
+    const uint8_t* scales;
+    bool four_bit;
+    int64_t rows;
+};
+
 template <int BN>
-lm_status launch(const CUtensorMap& map_w, const uint8_t* x, int64_t rows, int64_t cols, Args a, int64_t tiles, cudaStream_t stream) {
+lm_status launch(const Matrix& w, const Matrix& x, int64_t k, const Args& a, int64_t tiles, cudaStream_t stream) {
     using C = Cfg<BN>;
-    CUtensorMap map_x;
+    CUtensorMap map_w, map_x, map_ws, map_xs;
     std::string error;
-    if (!encode_tensor_map_mx(&map_x, x, a.x_four_bit != 0, static_cast<uint64_t>(rows), static_cast<uint64_t>(cols), BN, error))
-        return context_free_fail(LM_ERR_CUDA, error.c_str());
+    const uint64_t cols = static_cast<uint64_t>(mx_padded_cols(k)), pitch = static_cast<uint64_t>(mx_scale_pitch(k));
+    const auto encode = [&](const Matrix& m, uint32_t box, CUtensorMap* codes, CUtensorMap* scales) {
+        return encode_tensor_map_mx(codes, m.codes, m.four_bit, static_cast<uint64_t>(m.rows), cols, box, error) &&
+               encode_tensor_map_mx_scales(scales, m.scales, static_cast<uint64_t>(m.rows), pitch, box, kChunkBytes, error);
+    };
+    if (!encode(w, kBlockM, &map_w, &map_ws) || !encode(x, BN, &map_x, &map_xs)) return context_free_fail(LM_ERR_CUDA, error.c_str());
     if (const cudaError_t e = cudaFuncSetAttribute(mx_matmul_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes); e != cudaSuccess)
         return context_free_finish(e);
-    mx_matmul_kernel<BN><<<static_cast<unsigned>(std::min<int64_t>(tiles, kSms)), kThreads, C::kSmemBytes, stream>>>(map_w, map_x, a);
+    mx_matmul_kernel<BN><<<static_cast<unsigned>(std::min<int64_t>(tiles, kSms)), kThreads, C::kSmemBytes, stream>>>(map_w, map_x, map_ws, map_xs,
+                                                                                                                          a);
     return context_free_finish(cudaGetLastError());
 }
 
@@ -361,41 +396,34 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
     if (out == nullptr || !aligned(out, elem_size(out_dtype)) || !aligned(offsets, 4) || x == nullptr || x_scales == nullptr || w == nullptr || w_scales == nullptr ||
         !aligned(x, 32) || !aligned(x_scales, 16) || !aligned(w, 32) || !aligned(w_scales, 16))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_mx_matmul: a null pointer, or data not 32-byte or scales not 16-byte aligned");
-    // The tile's width: the average rows of a group, so that a group is one tile where that is cheap.
+    // The tile's width: groups are ragged, so half as much again as the average rows of a group keeps
+    // most of them in one tile (a second tile reads the group's weights again).
     const int64_t each = (rows + groups - 1) / groups;
-    const int bn = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : 128;
+    const int bn = each <= 10 ? 16 : each <= 20 ? 32 : each <= 40 ? 64 : 128;
     const int64_t m_blocks = (n + kBlockM - 1) / kBlockM;
     const int64_t column_tiles = (rows + bn - 1) / bn + std::min<int64_t>(groups, rows) - 1;  // at most
     if (column_tiles * m_blocks > INT32_MAX - kSms) return context_free_fail(LM_ERR_UNSUPPORTED, "lm_mx_matmul: more than 2^31 tiles");
     Args a{};
-    a.x_scales = x_scales;
-    a.w_scales = w_scales;
     a.offsets = offsets;
     a.out = out;
     a.out_stride = out_stride;
-    a.scale_pitch = mx_scale_pitch(k);
-    a.w_rows = groups * n;
     a.rows = static_cast<int>(rows);
     a.groups = groups;
     a.n = static_cast<int>(n);
-    a.k_stages = static_cast<int>(mx_padded_cols(k) / kStageCols);
+    a.k_boxes = static_cast<int>(mx_padded_cols(k) / kBoxCols);
     a.x_four_bit = x_format == LM_MX_E2M1;
     a.out_dtype = out_dtype;
     void* status = nullptr;
     if (const cudaError_t e = cudaGetSymbolAddress(&status, g_status); e != cudaSuccess) return context_free_finish(e);
     a.status = static_cast<int*>(status);
-    const int64_t cols = mx_padded_cols(k);
-    CUtensorMap map_w;
-    std::string error;
-    if (!encode_tensor_map_mx(&map_w, w, true, static_cast<uint64_t>(a.w_rows), static_cast<uint64_t>(cols), kBlockM, error))
-        return context_free_fail(LM_ERR_CUDA, error.c_str());
+    const Matrix mw{w, w_scales, true, groups * n}, mx{x, x_scales, x_format == LM_MX_E2M1, rows};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int64_t tiles = column_tiles * m_blocks;
     switch (bn) {
-        case 16: return launch<16>(map_w, x, rows, cols, a, tiles, s);
-        case 32: return launch<32>(map_w, x, rows, cols, a, tiles, s);
-        case 64: return launch<64>(map_w, x, rows, cols, a, tiles, s);
-        default: return launch<128>(map_w, x, rows, cols, a, tiles, s);
+        case 16: return launch<16>(mw, mx, k, a, tiles, s);
+        case 32: return launch<32>(mw, mx, k, a, tiles, s);
+        case 64: return launch<64>(mw, mx, k, a, tiles, s);
+        default: return launch<128>(mw, mx, k, a, tiles, s);
     }
 }
 
