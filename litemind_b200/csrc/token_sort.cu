@@ -8,8 +8,7 @@
 // atomics, so the same input always gives the same rows.
 #include "moe_internal.h"
 #include "elem.cuh"
-
-#include <algorithm>
+#include "ptx.cuh"
 
 namespace lm {
 namespace {
@@ -17,34 +16,68 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kPlanMaxExperts = 1024;
+constexpr int kPlanMaxCluster = 8;
+constexpr int kRowThreads = 256;
+constexpr int kRowWarps = kRowThreads / 32;
 
-// One CTA.  Each warp takes a contiguous run of pairs and counts them per expert in its own
-// histogram; a scan over (expert, warp) turns the counts into first rows; a second pass over the
-// run hands the rows out in order.
+// This CTA's `v[i]` (shared memory) as seen by the cluster's CTA `rank`.
+__device__ __forceinline__ int ld_cluster(const int* v, uint32_t rank) {
+    int r;
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(r) : "r"(mapa_shared(smem_u32(v), rank)) : "memory");
+    return r;
+}
+
+// One cluster.  Each warp takes a contiguous run of pairs and counts them per expert in its own
+// histogram; a scan over (expert, CTA, warp) turns the counts into first rows; a second pass over
+// the run hands the rows out in order.  The CTAs read one another's totals through distributed
+// shared memory, so that no workspace is needed and two plans at once share nothing.
 __global__ void __launch_bounds__(kPlanThreads)
-    sort_plan_kernel(const int32_t* __restrict__ idx, int64_t pairs, int experts, int32_t* __restrict__ offsets,
-                     int32_t* __restrict__ at) {
-    extern __shared__ int hist[];  // [warp][expert]
+    sort_plan_kernel(const int32_t* __restrict__ idx, int64_t pairs, int experts, int32_t* __restrict__ offsets, int32_t* __restrict__ at) {
+    extern __shared__ int hist[];  // [warp][expert], then this CTA's totals [expert]
     __shared__ int scan[kPlanWarps];
+    int* totals = hist + kPlanWarps * experts;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int rank = static_cast<int>(cluster_ctarank()), ctas = static_cast<int>(gridDim.x);
     for (int i = threadIdx.x; i < kPlanWarps * experts; i += kPlanThreads) hist[i] = 0;
     __syncthreads();
-    const int64_t groups = (pairs + 31) / 32;
-    const int64_t g0 = groups * warp / kPlanWarps, g1 = groups * (warp + 1) / kPlanWarps;
+    const int64_t groups = (pairs + 31) / 32, runs = static_cast<int64_t>(ctas) * kPlanWarps, run = static_cast<int64_t>(rank) * kPlanWarps + warp;
+    const int64_t g0 = groups * run / runs, g1 = groups * (run + 1) / runs;
     int* mine = hist + warp * experts;
-    for (int64_t g = g0; g < g1; ++g) {
+    const auto load = [&](int64_t g) {
         const int64_t p = g * 32 + lane;
-        const int e = p < pairs ? idx[p] : -1;
-        const unsigned same = __match_any_sync(0xffffffffu, e);
-        if (e >= 0 && e < experts && __ffs(same) - 1 == lane) mine[e] += __popc(same);
+        const int x = g < g1 && p < pairs ? idx[p] : -1;
+        return x < experts ? x : -1;
+    };
+    int x = load(g0), next = load(g0 + 1);
+    for (int64_t g = g0; g < g1; ++g) {
+        const int after = load(g + 2);
+        const unsigned same = __match_any_sync(0xffffffffu, x);
+        if (x >= 0 && __ffs(same) - 1 == lane) mine[x] += __popc(same);
         __syncwarp();
+        x = next, next = after;
     }
     __syncthreads();
-    // Thread e: its expert's total, then the exclusive scan over experts, then each warp's first row.
-    int total = 0;
+    // Thread e: its expert's total here and in the other CTAs, the exclusive scan over experts, and
+    // then the first row of each of this CTA's warps.
     const int e = threadIdx.x;
-    if (e < experts)
-        for (int w = 0; w < kPlanWarps; ++w) total += hist[w * experts + e];
+    int here = 0;
+    if (e < experts) {
+        for (int w = 0; w < kPlanWarps; ++w) here += hist[w * experts + e];
+        totals[e] = here;
+    }
+    int before = 0, total = here;
+    if (ctas > 1) {
+        cluster_sync();
+        if (e < experts) {
+            total = 0;
+            for (int c = 0; c < ctas; ++c) {
+                const int t = ld_cluster(&totals[e], static_cast<uint32_t>(c));
+                if (c < rank) before += t;
+                total += t;
+            }
+        }
+        cluster_sync();  // a CTA may not end while another reads its totals
+    }
     int incl = total;
     for (int d = 1; d < 32; d <<= 1) {
         const int o = __shfl_up_sync(0xffffffffu, incl, d);
@@ -63,8 +96,11 @@ __global__ void __launch_bounds__(kPlanThreads)
     __syncthreads();
     int first = incl - total + (warp > 0 ? scan[warp - 1] : 0);
     if (e < experts) {
-        offsets[e] = first;
-        if (e == experts - 1) offsets[experts] = first + total;
+        if (rank == 0) {
+            offsets[e] = first;
+            if (e == experts - 1) offsets[experts] = first + total;
+        }
+        first += before;
         for (int w = 0; w < kPlanWarps; ++w) {
             const int c = hist[w * experts + e];
             hist[w * experts + e] = first;
@@ -72,85 +108,177 @@ __global__ void __launch_bounds__(kPlanThreads)
         }
     }
     __syncthreads();
+    x = load(g0), next = load(g0 + 1);
     for (int64_t g = g0; g < g1; ++g) {
+        const int after = load(g + 2);
         const int64_t p = g * 32 + lane;
-        const int x = p < pairs ? idx[p] : -1;
         const unsigned same = __match_any_sync(0xffffffffu, x);
-        const bool live = x >= 0 && x < experts;
-        const int row = live ? mine[x] + __popc(same & ((1u << lane) - 1u)) : -1;
+        const int row = x >= 0 ? mine[x] + __popc(same & ((1u << lane) - 1u)) : -1;
         __syncwarp();
-        if (live && __ffs(same) - 1 == lane) mine[x] += __popc(same);
+        if (x >= 0 && __ffs(same) - 1 == lane) mine[x] += __popc(same);
         __syncwarp();
         if (p < pairs) at[p] = row;
+        x = next, next = after;
     }
 }
 
-// A CTA a token: its row is read once and written to each of its pairs' rows.
+// A warp takes 32 x kUnits units of a token's row: it reads them once, all loads in flight, and
+// writes them to each of the pairs' rows.
 template <class U>
-__global__ void __launch_bounds__(256)
-    sort_rows_kernel(const uint8_t* __restrict__ x, int64_t x_stride, const int32_t* __restrict__ at, int k, int64_t units,
+__global__ void __launch_bounds__(kRowThreads)
+    sort_rows_kernel(const uint8_t* __restrict__ x, int64_t x_stride, const int32_t* __restrict__ at, int64_t tokens, int k, int64_t units, int parts,
                      uint8_t* __restrict__ rows, int64_t rows_stride, int64_t n_rows) {
-    const int64_t t = blockIdx.x;
-    for (int64_t u = threadIdx.x; u < units; u += 256) {
-        const U v = reinterpret_cast<const U*>(x + t * x_stride)[u];
-        for (int j = 0; j < k; ++j) {
-            const int r = at[t * k + j];
-            if (r >= 0 && r < n_rows) reinterpret_cast<U*>(rows + r * rows_stride)[u] = v;
+    constexpr int kUnits = 4;
+    const int lane = threadIdx.x & 31;
+    const int64_t w = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5), t = w / parts;
+    if (t >= tokens) return;
+    const int64_t u0 = (w - t * parts) * (32 * kUnits) + lane;
+    const U* src = reinterpret_cast<const U*>(x + t * x_stride);
+    U v[kUnits];
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i)
+        if (u0 + 32 * i < units) v[i] = src[u0 + 32 * i];
+    for (int j0 = 0; j0 < k; j0 += 32) {
+        const int mine = j0 + lane < k ? at[t * k + j0 + lane] : -1;
+        for (int j = 0; j < min(32, k - j0); ++j) {
+            const int r = __shfl_sync(0xffffffffu, mine, j);
+            if (r < 0 || r >= n_rows) continue;
+            U* dst = reinterpret_cast<U*>(rows + r * rows_stride);
+#pragma unroll
+            for (int i = 0; i < kUnits; ++i)
+                if (u0 + 32 * i < units) dst[u0 + 32 * i] = v[i];
         }
     }
 }
 
-// A CTA a token: y = sum over slots in order, in f32, rounded once.
-template <int DT, int DY>
-__global__ void __launch_bounds__(256)
+// V consecutive values of a row from column c on; V is 8 for rows of whole 16-byte words, else 1.
+template <int DT, int V>
+__device__ __forceinline__ void load_row(const typename Elem<DT>::T* p, float (&v)[V]) {
+    if constexpr (V == 8) load8<DT>(p, v);
+    else v[0] = Elem<DT>::widen(*p);
+}
+template <int DT, int V>
+__device__ __forceinline__ void store_row(typename Elem<DT>::T* p, const float (&v)[V]) {
+    if constexpr (V == 8) store8<DT>(p, v);
+    else *p = Elem<DT>::narrow(v[0]);
+}
+
+constexpr int kSlots = 4;  // rows whose loads are in flight together
+
+// A warp takes 32 V columns of a token: y = the sum over its slots in order, in f32, rounded once.
+template <int DT, int DY, int V>
+__global__ void __launch_bounds__(kRowThreads)
     unsort_rows_kernel(const typename Elem<DT>::T* __restrict__ rows, int64_t n_rows, const int32_t* __restrict__ at,
-                       const float* __restrict__ weights, int k, int64_t cols, typename Elem<DY>::T* __restrict__ y, bool accumulate) {
-    const int64_t t = blockIdx.x;
-    for (int64_t c = threadIdx.x; c < cols; c += 256) {
-        float s = 0.0f;
-        for (int j = 0; j < k; ++j) {
-            const int r = at[t * k + j];
-            if (r >= 0 && r < n_rows) {
-                const float v = Elem<DT>::widen(rows[r * cols + c]);
-                s = weights != nullptr ? fmaf(weights[t * k + j], v, s) : s + v;
+                       const float* __restrict__ weights, int64_t tokens, int k, int64_t cols, int parts, typename Elem<DY>::T* __restrict__ y,
+                       int accumulate) {
+    const int lane = threadIdx.x & 31;
+    const int64_t w = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5), t = w / parts;
+    if (t >= tokens) return;
+    const int64_t c = ((w - t * parts) * 32 + lane) * V;
+    const bool live = c < cols;
+    float s[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] = 0.0f;
+    for (int j0 = 0; j0 < k; j0 += 32) {
+        const int my_row = j0 + lane < k ? at[t * k + j0 + lane] : -1;
+        const float my_weight = weights != nullptr && j0 + lane < k ? weights[t * k + j0 + lane] : 1.0f;
+        for (int j = 0; j < min(32, k - j0); j += kSlots) {
+            float v[kSlots][V];
+            bool has[kSlots];
+#pragma unroll
+            for (int q = 0; q < kSlots; ++q) {
+                const int r = __shfl_sync(0xffffffffu, my_row, (j + q) & 31);
+                has[q] = j + q < 32 && r >= 0 && r < n_rows && live;
+                if (has[q]) load_row<DT, V>(rows + r * cols + c, v[q]);
+            }
+#pragma unroll
+            for (int q = 0; q < kSlots; ++q) {
+                const float weight = __shfl_sync(0xffffffffu, my_weight, (j + q) & 31);
+                if (has[q]) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) s[i] = fmaf(weight, v[q][i], s[i]);
+                }
             }
         }
-        if (accumulate) s += Elem<DY>::widen(y[t * cols + c]);
-        y[t * cols + c] = Elem<DY>::narrow(s);
+    }
+    if (!live) return;
+    typename Elem<DY>::T* dst = y + t * cols + c;
+    if (accumulate) {
+        float v[V];
+        load_row<DY, V>(dst, v);
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] += v[i];
+    }
+    store_row<DY, V>(dst, s);
+}
+
+// grad_rows[at] = w grad_y, grad_weights = <grad_y, rows[at]> (0 for a dropped pair).  W warps take
+// a token's columns in turns, kSlots slots at a time, and add their dot products at the end.
+template <int DT, int V, int W>
+__global__ void __launch_bounds__(kRowThreads)
+    unsort_rows_backward_kernel(const typename Elem<DT>::T* __restrict__ grad_y, const typename Elem<DT>::T* rows, int64_t n_rows,
+                                const int32_t* __restrict__ at, const float* __restrict__ weights, int64_t tokens, int k, int64_t cols,
+                                typename Elem<DT>::T* grad_rows, float* __restrict__ grad_weights) {
+    __shared__ float red[kRowWarps][kSlots];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t t = static_cast<int64_t>(blockIdx.x) * (kRowWarps / W) + warp / W;
+    if (t >= tokens) return;
+    for (int j0 = 0; j0 < k; j0 += kSlots) {
+        int r[kSlots];
+        float weight[kSlots], dot[kSlots];
+#pragma unroll
+        for (int q = 0; q < kSlots; ++q) {
+            r[q] = j0 + q < k ? at[t * k + j0 + q] : -1;
+            if (r[q] >= n_rows) r[q] = -1;
+            weight[q] = r[q] >= 0 ? weights[t * k + j0 + q] : 0.0f;
+            dot[q] = 0.0f;
+        }
+        for (int64_t c = (warp % W * 32 + lane) * V; c < cols; c += W * 32 * V) {
+            float g[V], v[kSlots][V];
+            load_row<DT, V>(grad_y + t * cols + c, g);
+#pragma unroll
+            for (int q = 0; q < kSlots; ++q)
+                if (r[q] >= 0) load_row<DT, V>(rows + r[q] * cols + c, v[q]);
+#pragma unroll
+            for (int q = 0; q < kSlots; ++q) {
+                if (r[q] < 0) continue;
+                float out[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    dot[q] = fmaf(g[i], v[q][i], dot[q]);
+                    out[i] = weight[q] * g[i];
+                }
+                store_row<DT, V>(grad_rows + r[q] * cols + c, out);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < kSlots; ++q)
+            for (int off = 16; off > 0; off >>= 1) dot[q] += __shfl_xor_sync(0xffffffffu, dot[q], off);
+        if constexpr (W > 1) {
+            if (lane == 0)
+                for (int q = 0; q < kSlots; ++q) red[warp][q] = dot[q];
+            __syncthreads();
+            if (threadIdx.x < kSlots && j0 + threadIdx.x < k) {
+                float s = 0.0f;
+                for (int i = 0; i < W; ++i) s += red[i][threadIdx.x];
+                grad_weights[t * k + j0 + threadIdx.x] = s;
+            }
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int q = 0; q < kSlots; ++q)
+                if (lane == q && j0 + q < k) grad_weights[t * k + j0 + q] = dot[q];
+        }
     }
 }
 
-// A CTA a token: grad_rows[at] = w grad_y, grad_weights = <grad_y, rows[at]> (0 for a dropped pair).
-template <int DT>
-__global__ void __launch_bounds__(256)
-    unsort_rows_backward_kernel(const typename Elem<DT>::T* __restrict__ grad_y, const typename Elem<DT>::T* rows,
-                                int64_t n_rows, const int32_t* __restrict__ at, const float* __restrict__ weights, int k, int64_t cols,
-                                typename Elem<DT>::T* grad_rows, float* __restrict__ grad_weights) {
-    __shared__ float red[8];
-    const int64_t t = blockIdx.x;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int j = 0; j < k; ++j) {
-        const int r = at[t * k + j];
-        const bool live = r >= 0 && r < n_rows;
-        const float w = weights[t * k + j];
-        float s = 0.0f;
-        if (live) {
-            for (int64_t c = threadIdx.x; c < cols; c += 256) {
-                const float g = Elem<DT>::widen(grad_y[t * cols + c]);
-                s = fmaf(g, Elem<DT>::widen(rows[r * cols + c]), s);
-                grad_rows[r * cols + c] = Elem<DT>::narrow(w * g);
-            }
-        }
-        for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        if (lane == 0) red[warp] = s;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            float a = 0.0f;
-            for (int i = 0; i < 8; ++i) a += red[i];
-            grad_weights[t * k + j] = a;
-        }
-        __syncthreads();
-    }
+// A launch of one warp for each (token, part of its row).
+template <class F>
+lm_status with_parts(int64_t tokens, int64_t parts, F&& f) {
+    const int64_t blocks = (tokens * parts + kRowWarps - 1) / kRowWarps;
+    if (parts > INT32_MAX || blocks > INT32_MAX) return context_free_fail(LM_ERR_UNSUPPORTED, "rows of more than 2^44 bytes in all");
+    f(static_cast<unsigned>(blocks), static_cast<int>(parts));
+    return context_free_finish(cudaGetLastError());
 }
 
 bool sizes_ok(int64_t tokens, int32_t k) {
@@ -170,13 +298,27 @@ lm_status lm_moe_sort_plan(const int32_t* topk_idx, int64_t tokens, int32_t top_
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_sort_plan: tokens x top_k beyond 2^31, top_k beyond 64 or experts beyond 1024");
     if (offsets == nullptr || !aligned(offsets, 4) || (tokens > 0 && (topk_idx == nullptr || at == nullptr || !aligned(topk_idx, 4) || !aligned(at, 4))))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_sort_plan: a null or misaligned pointer");
-    const int smem = kPlanWarps * experts * 4;
-    if (smem > 48 * 1024)
-        if (const cudaError_t e = cudaFuncSetAttribute(sort_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPlanWarps * kPlanMaxExperts * 4);
+    // A CTA for each 4096 pairs (four rounds of a warp's 32), up to a cluster of eight.
+    const int64_t pairs = tokens * top_k;
+    int ctas = 1;
+    while (ctas < kPlanMaxCluster && pairs > int64_t(4096) * ctas) ctas *= 2;
+    const int smem = (kPlanWarps + 1) * experts * 4;
+    if (smem > 40 * 1024)
+        if (const cudaError_t e = cudaFuncSetAttribute(sort_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kPlanWarps + 1) * kPlanMaxExperts * 4);
             e != cudaSuccess)
             return context_free_finish(e);
-    sort_plan_kernel<<<1, kPlanThreads, smem, static_cast<cudaStream_t>(stream)>>>(topk_idx, tokens * top_k, experts, offsets, at);
-    return context_free_finish(cudaGetLastError());
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+    cfg.blockDim = dim3(kPlanThreads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = static_cast<unsigned>(ctas);
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cfg.attrs = &cluster;
+    cfg.numAttrs = 1;
+    return context_free_finish(cudaLaunchKernelEx(&cfg, sort_plan_kernel, topk_idx, pairs, static_cast<int>(experts), offsets, at));
 }
 
 lm_status lm_moe_sort_rows(const void* x, int64_t x_stride, const int32_t* at, int64_t tokens, int32_t top_k, int64_t row_bytes, void* rows,
@@ -190,15 +332,16 @@ lm_status lm_moe_sort_rows(const void* x, int64_t x_stride, const int32_t* at, i
                           static_cast<uintptr_t>(rows_stride) | static_cast<uintptr_t>(row_bytes);
     const auto go = [&](auto unit) {
         using U = decltype(unit);
-        sort_rows_kernel<U><<<static_cast<unsigned>(tokens), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-            static_cast<const uint8_t*>(x), x_stride, at, top_k, row_bytes / static_cast<int64_t>(sizeof(U)), static_cast<uint8_t*>(rows), rows_stride,
-            n_rows);
+        const int64_t units = row_bytes / static_cast<int64_t>(sizeof(U));
+        return with_parts(tokens, (units + 127) / 128, [&](unsigned grid, int parts) {
+            sort_rows_kernel<U><<<grid, kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const uint8_t*>(x), x_stride, at, tokens, top_k, units, parts,
+                                                                                             static_cast<uint8_t*>(rows), rows_stride, n_rows);
+        });
     };
-    if (all % 16 == 0) go(uint4{});
-    else if (all % 4 == 0) go(uint32_t{});
-    else if (all % 2 == 0) go(uint16_t{});
-    else go(uint8_t{});
-    return context_free_finish(cudaGetLastError());
+    if (all % 16 == 0) return go(uint4{});
+    if (all % 4 == 0) return go(uint32_t{});
+    if (all % 2 == 0) return go(uint16_t{});
+    return go(uint8_t{});
 }
 
 lm_status lm_moe_unsort_rows(const void* rows, int32_t dtype, int64_t n_rows, const int32_t* at, const float* weights, int64_t tokens, int32_t top_k,
@@ -211,17 +354,22 @@ lm_status lm_moe_unsort_rows(const void* rows, int32_t dtype, int64_t n_rows, co
     if ((rows == nullptr && n_rows > 0) || at == nullptr || y == nullptr || !aligned(rows, elem_size(dtype)) || !aligned(y, elem_size(y_dtype)) || !aligned(at, 4) ||
         !aligned(weights, 4))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows: a null or misaligned pointer");
-    with_dtype(dtype, [&](auto dt) {
-        constexpr int DT = decltype(dt)::value;
-        const auto go = [&](auto dy) {
-            constexpr int DY = decltype(dy)::value;
-            unsort_rows_kernel<DT, DY><<<static_cast<unsigned>(tokens), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-                static_cast<const typename Elem<DT>::T*>(rows), n_rows, at, weights, top_k, cols, static_cast<typename Elem<DY>::T*>(y), accumulate != 0);
-        };
-        if (y_dtype == LM_DTYPE_F32) go(std::integral_constant<int, LM_DTYPE_F32>{});
-        else go(dt);
+    const bool vec = cols % 8 == 0 && aligned(rows, 16) && aligned(y, 16);
+    return with_parts(tokens, (cols + (vec ? 255 : 31)) / (vec ? 256 : 32), [&](unsigned grid, int parts) {
+        with_dtype(dtype, [&](auto dt) {
+            with_bool(vec, [&](auto v) {
+                constexpr int DT = decltype(dt)::value, V = decltype(v)::value ? 8 : 1;
+                const auto go = [&](auto dy) {
+                    constexpr int DY = decltype(dy)::value;
+                    unsort_rows_kernel<DT, DY, V><<<grid, kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+                        static_cast<const typename Elem<DT>::T*>(rows), n_rows, at, weights, tokens, top_k, cols, parts, static_cast<typename Elem<DY>::T*>(y),
+                        accumulate != 0);
+                };
+                if (y_dtype == LM_DTYPE_F32) go(std::integral_constant<int, LM_DTYPE_F32>{});
+                else go(dt);
+            });
+        });
     });
-    return context_free_finish(cudaGetLastError());
 }
 
 lm_status lm_moe_unsort_rows_backward(const void* grad_y, const void* rows, int32_t dtype, int64_t n_rows, const int32_t* at, const float* weights,
@@ -234,11 +382,19 @@ lm_status lm_moe_unsort_rows_backward(const void* grad_y, const void* rows, int3
         !aligned(grad_y, elem_size(dtype)) || !aligned(rows, elem_size(dtype)) || !aligned(grad_rows, elem_size(dtype)) || !aligned(at, 4) || !aligned(weights, 4) ||
         !aligned(grad_weights, 4))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows_backward: a null or misaligned pointer");
+    const bool vec = cols % 8 == 0 && aligned(grad_y, 16) && aligned(rows, 16) && aligned(grad_rows, 16);
+    // A warp a token when that fills the GPU, else all eight warps of a CTA.
+    const bool wide = tokens < 148 * 4 * kRowWarps;
     with_dtype(dtype, [&](auto dt) {
-        constexpr int DT = decltype(dt)::value;
-        using T = typename Elem<DT>::T;
-        unsort_rows_backward_kernel<DT><<<static_cast<unsigned>(tokens), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-            static_cast<const T*>(grad_y), static_cast<const T*>(rows), n_rows, at, weights, top_k, cols, static_cast<T*>(grad_rows), grad_weights);
+        with_bool(vec, [&](auto v) {
+            with_bool(wide, [&](auto wd) {
+                constexpr int DT = decltype(dt)::value, W = decltype(wd)::value ? kRowWarps : 1, per = kRowWarps / W;
+                using T = typename Elem<DT>::T;
+                unsort_rows_backward_kernel<DT, decltype(v)::value ? 8 : 1, W>
+                    <<<static_cast<unsigned>((tokens + per - 1) / per), kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+                        static_cast<const T*>(grad_y), static_cast<const T*>(rows), n_rows, at, weights, tokens, top_k, cols, static_cast<T*>(grad_rows), grad_weights);
+            });
+        });
     });
     return context_free_finish(cudaGetLastError());
 }
