@@ -450,10 +450,10 @@ lm_status lm_mx_dequantize(const uint8_t* data, const uint8_t* scales, int32_t f
 lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_format, int64_t rows, const uint8_t* w,
                        const uint8_t* w_scales, int32_t groups, int64_t n, int64_t k, const int32_t* offsets, void* out,
                        int32_t out_dtype, int64_t out_stride, void* stream);
-/* Waits for the stream and reports a device-side timeout of an lm_mx_matmul on the current device
- * since the last call (then clears it), as lm_moe_sync does for a context: LM_ERR_DEVICE_TIMEOUT,
- * and the results of the products since then are invalid. */
-lm_status lm_mx_sync(void* stream);
+/* Waits for the stream and reports a device-side timeout of the operators without a context
+ * (lm_mx_matmul) on the current device since the last call, then clears it, as lm_moe_sync does for a context: LM_ERR_DEVICE_TIMEOUT, and the results of
+ * the calls since then are invalid. */
+lm_status lm_ops_sync(void* stream);
 
 /* ── gemm:: kernels on device memory (include/Gemm.hpp:23-72) ──────────────── */
 

@@ -103,7 +103,7 @@ SIGNATURES = {
     "lm_mx_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp, _vp]),
     "lm_mx_dequantize": (_i32, [_vp, _vp, _i32, _i64, _i64, _vp, _i32, _i64, _vp]),
     "lm_mx_matmul": (_i32, [_vp, _vp, _i32, _i64, _vp, _vp, _i32, _i64, _i64, _vp, _vp, _i32, _i64, _vp]),
-    "lm_mx_sync": (_i32, [_vp]),
+    "lm_ops_sync": (_i32, [_vp]),
     "lm_gemm_add_rms_norm_mx": (_i32, [_vp, _i32, _vp, _i32, _vp, _i64, _i64, _f32, _vp, _vp, _i32, _vp, _vp, _vp]),
     "lm_kernel_description": (C.c_char_p, []),
     "lm_gemm_matvec_bf16": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp]),

@@ -69,6 +69,26 @@ __device__ __forceinline__ void store8(typename Elem<DT>::T* p, const float (&v)
     }
 }
 
+// Eight elements as they lie in memory: half the registers of their f32 values for 16-bit types
+// while loads are in flight.
+template <int DT>
+struct Raw8 {
+    uint32_t w[2 * sizeof(typename Elem<DT>::T)];
+    __device__ __forceinline__ void load(const typename Elem<DT>::T* p) {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(w) / 16); ++i) {
+            const uint4 q = reinterpret_cast<const uint4*>(p)[i];
+            w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+        }
+    }
+    __device__ __forceinline__ void widen(float (&v)[8]) const {
+        typename Elem<DT>::T e[8];
+        memcpy(e, w, sizeof e);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = Elem<DT>::widen(e[i]);
+    }
+};
+
 // ── entry points ─────────────────────────────────────────────────────────
 inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 inline int64_t elem_size(int32_t dtype) { return dtype == LM_DTYPE_F32 ? 4 : 2; }

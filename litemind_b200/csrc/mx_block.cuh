@@ -29,17 +29,40 @@ inline int64_t mx_scale_pitch(int64_t cols) { return (cols + 511) / 512 * 16; }
 template <int FMT>
 constexpr int kMxEmax = FMT == LM_MX_E2M1 ? 2 : 8;
 
+// The scale byte of a block whose largest magnitude has these f32 bits.
+template <int FMT>
+__device__ __forceinline__ uint32_t mx_scale_of(uint32_t top) {
+    if (top >= 0x7f800000u) return 255u;
+    return static_cast<uint32_t>(max(static_cast<int>(top >> 23) - kMxEmax<FMT>, 0));
+}
 // The scale byte of the block that lanes 4i..4i+3 of this warp hold (all 32 lanes call it).
+// Magnitudes order as their bits do, infinities and NaN above all.
 template <int FMT>
 __device__ __forceinline__ uint32_t mx_scale_byte(const float (&v)[8]) {
-    uint32_t top = 0;  // magnitudes order as their bits do, infinities and NaN above all
+    uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    if (top >= 0x7f800000u) return 255u;
-    const int e = static_cast<int>(top >> 23) - kMxEmax<FMT>;
-    return static_cast<uint32_t>(max(e, 0));
+    return mx_scale_of<FMT>(top);
+}
+// The same from the elements as they lie: 16-bit types two at a time.
+template <int FMT, int DT>
+__device__ __forceinline__ uint32_t mx_scale_byte(const Raw8<DT>& r) {
+    if constexpr (DT == LM_DTYPE_F32) {
+        float v[8];
+        r.widen(v);
+        return mx_scale_byte<FMT>(v);
+    } else {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = __vmaxu2(top, r.w[i] & 0x7fff7fffu);
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        top = max(top & 0xffffu, top >> 16);
+        if constexpr (DT == LM_DTYPE_BF16) return mx_scale_of<FMT>(top << 16);
+        else return mx_scale_of<FMT>(__float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(top)))));
+    }
 }
 
 // This lane's eight codes: 32 bits of E2M1, or 64 of E4M3 in (x, y).

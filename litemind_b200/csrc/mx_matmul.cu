@@ -14,7 +14,7 @@
 //   8-11   epilogue: TMEM to registers to out, rounded once; double buffered against the MMA
 // A stage costs the issuer about 400 cycles of waits, descriptors and commits whatever its width,
 // and four MMAs take 200 (N = 16) to 256 (N = 128): hence eight of them a stage.
-// Every wait is bounded (ptx.cuh): a pipeline that stalls records a status for lm_mx_sync.
+// Every wait is bounded (ptx.cuh): a pipeline that stalls records a status for lm_ops_sync.
 #include "moe_internal.h"
 #include "mx_block.cuh"
 #include "ptx.cuh"
@@ -59,7 +59,7 @@ struct Args {
     int* status;
 };
 
-__device__ int g_status;  // the first device-side error since the last lm_mx_sync
+__device__ int g_status;  // the first device-side error since the last lm_ops_sync
 
 // Where group g's rows start (cut[g]) and its first column tile (tiles[g]); one warp.  Offsets are
 // clamped to the rows and to ascending order, so no value of theirs leads outside the matrices.
@@ -378,6 +378,14 @@ lm_status launch(const Matrix& w, const Matrix& x, int64_t k, const Args& a, int
 }
 
 }  // namespace
+
+cudaError_t ops_status(int** status) {
+    void* p = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&p, g_status);
+    *status = static_cast<int*>(p);
+    return e;
+}
+
 }  // namespace lm
 
 using namespace lm;
@@ -413,9 +421,7 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
     a.k_boxes = static_cast<int>(mx_padded_cols(k) / kBoxCols);
     a.x_four_bit = x_format == LM_MX_E2M1;
     a.out_dtype = out_dtype;
-    void* status = nullptr;
-    if (const cudaError_t e = cudaGetSymbolAddress(&status, g_status); e != cudaSuccess) return context_free_finish(e);
-    a.status = static_cast<int*>(status);
+    if (const cudaError_t e = ops_status(&a.status); e != cudaSuccess) return context_free_finish(e);
     const Matrix mw{w, w_scales, true, groups * n}, mx{x, x_scales, x_format == LM_MX_E2M1, rows};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int64_t tiles = column_tiles * m_blocks;
@@ -427,7 +433,7 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
     }
 }
 
-lm_status lm_mx_sync(void* stream) {
+lm_status lm_ops_sync(void* stream) {
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     int code = 0;
     cudaError_t e = cudaMemcpyFromSymbolAsync(&code, g_status, sizeof code, 0, cudaMemcpyDeviceToHost, s);
@@ -438,7 +444,7 @@ lm_status lm_mx_sync(void* stream) {
     e = cudaMemcpyToSymbolAsync(g_status, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, s);
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
     if (e != cudaSuccess) return context_free_finish(e);
-    return context_free_fail(LM_ERR_DEVICE_TIMEOUT, "lm_mx_sync: a product gave up waiting; its results are invalid");
+    return context_free_fail(LM_ERR_DEVICE_TIMEOUT, "lm_ops_sync: a kernel gave up waiting; its results are invalid");
 }
 
 }  // extern "C"

@@ -16,13 +16,10 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kSegCols = 256;  // columns a warp takes at a time: 8 a lane, 8 blocks of 32
 constexpr int kFlight = 4;     // segments a warp has in flight
 
-// Segments of all rows, laid end to end; a warp takes kFlight of them, kWarps apart, at a time.
-// I is the type of a segment's number: 32 bits where they fit, since a 64-bit division for each
-// segment costs as much as its conversion.
-template <class I>
-__device__ __forceinline__ I first_segment() {
-    return static_cast<I>(blockIdx.x) * (kWarps * kFlight) + (threadIdx.x >> 5);
-}
+// A warp takes kFlight segments of one row: block (x, y) holds rows kWarps x .. and segments
+// kFlight y .. of each, so that no index needs a division (divisions cost as much as the conversion).
+__device__ __forceinline__ int64_t warp_row() { return static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); }
+__device__ __forceinline__ int64_t first_col() { return static_cast<int64_t>(blockIdx.y) * (kFlight * kSegCols) + (threadIdx.x & 31) * 8; }
 
 // Eight values from column `col` on; zeros past the row's end.
 template <int DT, bool VEC>
@@ -33,6 +30,19 @@ __device__ __forceinline__ void load_cols(const typename Elem<DT>::T* row, int64
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? Elem<DT>::widen(row[col + i]) : 0.0f;
     }
+}
+template <int DT, bool VEC>
+__device__ __forceinline__ Raw8<DT> load_raw(const typename Elem<DT>::T* row, int64_t col, int64_t cols) {
+    Raw8<DT> r;
+    if (VEC && col + 8 <= cols) {
+        r.load(row + col);
+    } else {
+        typename Elem<DT>::T e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = col + i < cols ? row[col + i] : Elem<DT>::narrow(0.0f);
+        memcpy(r.w, e, sizeof e);
+    }
+    return r;
 }
 template <int DT, bool VEC>
 __device__ __forceinline__ void store_cols(typename Elem<DT>::T* row, int64_t col, int64_t cols, const float (&v)[8]) {
@@ -55,81 +65,97 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int64_t col, int64_t d
     else *reinterpret_cast<uint2*>(row + at) = codes;
 }
 
-// A warp takes a segment of a row: 256 columns, 8 scale bytes.  `segs` covers the padded scales,
-// so the last segments of a row may hold scale padding only.
-template <int DT, int FMT, bool VEC, class I>
+// Each segment has 8 scale bytes; the last ones of a row may be padding only.
+template <int DT, int FMT, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-    mx_quantize_kernel(const typename Elem<DT>::T* __restrict__ values, I total, int64_t cols, int64_t row_stride, int segs,
-                       uint8_t* __restrict__ data, int64_t data_pitch, uint8_t* __restrict__ scales) {
+    mx_quantize_kernel(const typename Elem<DT>::T* __restrict__ values, int64_t rows, int64_t cols, int64_t row_stride, uint8_t* __restrict__ data,
+                       int64_t data_pitch, uint8_t* __restrict__ scales, int64_t scale_pitch) {
     const int lane = threadIdx.x & 31;
-    const I w0 = first_segment<I>();
-    float v[kFlight][8];
+    const int64_t row = warp_row(), col0 = first_col();
+    if (row >= rows) return;
+    values += row * row_stride, data += row * data_pitch, scales += row * scale_pitch;
+    Raw8<DT> raw[kFlight];
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) raw[f] = load_raw<DT, VEC>(values, col0 + f * kSegCols, cols);
 #pragma unroll
     for (int f = 0; f < kFlight; ++f) {
-        const I w = w0 + f * kWarps, row = w / segs;
-        const int64_t col = static_cast<int64_t>(w - row * segs) * kSegCols + lane * 8;
-        load_cols<DT, VEC>(values + row * row_stride, col, w < total ? cols : 0, v[f]);
-    }
-#pragma unroll
-    for (int f = 0; f < kFlight; ++f) {
-        const I w = w0 + f * kWarps, row = w / segs;
-        if (w >= total) break;
-        const int64_t col = static_cast<int64_t>(w - row * segs) * kSegCols + lane * 8;
-        const uint32_t byte = mx_scale_byte<FMT>(v[f]);
-        store_codes<FMT>(data + row * data_pitch, col, data_pitch, mx_encode8<FMT>(v[f], byte));
+        const int64_t col = col0 + f * kSegCols;
+        if (col >= scale_pitch * kMxBlock) break;  // the same for a whole warp: pitches are multiples of 8 bytes
+        const uint32_t byte = mx_scale_byte<FMT>(raw[f]);
+        float v[8];
+        raw[f].widen(v);
+        store_codes<FMT>(data, col, data_pitch, mx_encode8<FMT>(v, byte));
         const uint32_t word = mx_gather_scales(byte, lane);
-        if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + static_cast<int64_t>(w) * 8 + (lane >> 4) * 4) = word;
+        if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(scales + col / kMxBlock) = word;
     }
 }
 
-template <int DT, int FMT, bool VEC, class I>
+template <int DT, int FMT, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-    mx_dequantize_kernel(const uint8_t* __restrict__ data, int64_t data_pitch, const uint8_t* __restrict__ scales, int64_t scale_pitch, I total,
-                         int64_t cols, int segs, typename Elem<DT>::T* __restrict__ values, int64_t row_stride) {
-    const int lane = threadIdx.x & 31;
-    const I w0 = first_segment<I>();
+    mx_dequantize_kernel(const uint8_t* __restrict__ data, int64_t data_pitch, const uint8_t* __restrict__ scales, int64_t scale_pitch, int64_t rows,
+                         int64_t cols, typename Elem<DT>::T* __restrict__ values, int64_t row_stride) {
+    const int64_t row = warp_row(), col0 = first_col();
+    if (row >= rows) return;
+    values += row * row_stride;
+    if constexpr (!VEC) {
+        // Rows that do not start on whole words: lane i takes column i of each block, so that stores
+        // run along the row (8192 x 2047 to bf16 took 51 us with eight neighbouring columns a lane).
+        const int lane = threadIdx.x & 31;
+        data += row * data_pitch, scales += row * scale_pitch;
+        const int64_t col1 = min(cols, static_cast<int64_t>(blockIdx.y + 1) * (kFlight * kSegCols));
+#pragma unroll 8
+        for (int64_t col = static_cast<int64_t>(blockIdx.y) * (kFlight * kSegCols) + lane; col < col1; col += kMxBlock) {
+            uint32_t code = FMT == LM_MX_E2M1 ? data[col / 2] : data[col];
+            if (FMT == LM_MX_E2M1 && (col & 1)) code >>= 4;
+            float v[8];
+            mx_decode8<FMT>(make_uint2(code, 0u), scales[col / kMxBlock], v);
+            values[col] = Elem<DT>::narrow(v[0]);
+        }
+        return;
+    }
+    data += row * data_pitch + col0 * (FMT == LM_MX_E2M1 ? 4 : 8) / 8, scales += row * scale_pitch + col0 / kMxBlock;
     uint2 codes[kFlight];
     uint32_t byte[kFlight];
 #pragma unroll
     for (int f = 0; f < kFlight; ++f) {
-        const I w = w0 + f * kWarps, row = w / segs;
-        const int64_t col = static_cast<int64_t>(w - row * segs) * kSegCols + lane * 8;
         codes[f] = make_uint2(0u, 0u);
         byte[f] = 0;
-        if (w < total && col < cols) {
-            const uint8_t* src = data + row * data_pitch + col * (FMT == LM_MX_E2M1 ? 4 : 8) / 8;
-            if constexpr (FMT == LM_MX_E2M1) codes[f].x = *reinterpret_cast<const uint32_t*>(src);
-            else codes[f] = *reinterpret_cast<const uint2*>(src);
-            byte[f] = scales[row * scale_pitch + col / kMxBlock];
+        if (col0 + f * kSegCols < cols) {
+            if constexpr (FMT == LM_MX_E2M1) codes[f].x = *reinterpret_cast<const uint32_t*>(data + f * (kSegCols / 2));
+            else codes[f] = *reinterpret_cast<const uint2*>(data + f * kSegCols);
+            byte[f] = scales[f * (kSegCols / kMxBlock)];
         }
     }
 #pragma unroll
     for (int f = 0; f < kFlight; ++f) {
-        const I w = w0 + f * kWarps, row = w / segs;
-        if (w >= total) break;
-        const int64_t col = static_cast<int64_t>(w - row * segs) * kSegCols + lane * 8;
+        if (col0 + f * kSegCols >= cols) break;
         float v[8];
         mx_decode8<FMT>(codes[f], byte[f], v);
-        store_cols<DT, VEC>(values + row * row_stride, col, cols, v);
+        store_cols<DT, VEC>(values, col0 + f * kSegCols, cols, v);
     }
 }
 
-// The sum's eight values at `col`, rounded to the residual's type and stored, and their squares' sum.
+// Eight values of the residual and of its update; zeros for an update that is not there.
 template <int DT, bool VEC>
-__device__ __forceinline__ double add_store(const typename Elem<DT>::T* hidden, const void* delta, bool delta_f32, int64_t col, int64_t cols,
-                                           typename Elem<DT>::T* sum, float (&v)[8]) {
+__device__ __forceinline__ void load_pair(const typename Elem<DT>::T* hidden, const void* delta, bool delta_f32, int64_t col, int64_t cols, float (&v)[8],
+                                          float (&d)[8]) {
     load_cols<DT, VEC>(hidden, col, cols, v);
-    if (delta != nullptr) {
-        float d[8];
-        if (delta_f32) load_cols<LM_DTYPE_F32, VEC>(static_cast<const float*>(delta), col, cols, d);
-        else load_cols<LM_DTYPE_BF16, VEC>(static_cast<const __nv_bfloat16*>(delta), col, cols, d);
+    if (delta == nullptr) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += d[i];
+        for (int i = 0; i < 8; ++i) d[i] = 0.0f;
+    } else if (delta_f32) {
+        load_cols<LM_DTYPE_F32, VEC>(static_cast<const float*>(delta), col, cols, d);
+    } else {
+        load_cols<LM_DTYPE_BF16, VEC>(static_cast<const __nv_bfloat16*>(delta), col, cols, d);
     }
+}
+// Their sum, rounded to the residual's type and stored, in v; returns the sum of its squares.
+template <int DT, bool VEC>
+__device__ __forceinline__ double add_store(float (&v)[8], const float (&d)[8], bool add, int64_t col, int64_t cols, typename Elem<DT>::T* sum) {
     double s = 0.0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        v[i] = Elem<DT>::widen(Elem<DT>::narrow(v[i]));
+        if (add) v[i] = Elem<DT>::widen(Elem<DT>::narrow(v[i] + d[i]));
         s = fma(static_cast<double>(v[i]), static_cast<double>(v[i]), s);
     }
     store_cols<DT, VEC>(sum, col, cols, v);
@@ -156,48 +182,52 @@ __device__ __forceinline__ void put_norm(float (&v)[8], float inverse, const flo
     if ((threadIdx.x & 3) == 0) scales[col / kMxBlock] = static_cast<uint8_t>(byte);
 }
 
-// The sum of s over the `T` threads of a row.
+// The sum of s over the CTA.
 template <int T>
-__device__ __forceinline__ double row_sum(double s, double* red) {
+__device__ __forceinline__ double block_sum(double s) {
+    __shared__ double red[T / 32];
     for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    if constexpr (T > 32) {
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
-        __syncthreads();
-        s = 0.0;
-        for (int i = 0; i < T / 32; ++i) s += red[i];
-    }
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+    __syncthreads();
+    s = 0.0;
+#pragma unroll
+    for (int i = 0; i < T / 32; ++i) s += red[i];
     return s;
 }
 
-// T threads a row, eight columns each of every stretch of 8 T.  With CHUNKS > 0 that many
-// stretches stay in registers between the sum and the norm; CHUNKS = 0 reads the stored sum again
-// (each thread its own stores).  The sum is normalised as stored, its squares
-// added in f64 as lm_gemm_rms_norm adds them.
+// A CTA of T threads a row, eight columns a thread of every stretch of 8 T.  With CHUNKS > 0 that
+// many stretches are loaded before anything is stored (sum may be hidden or delta, so the compiler
+// cannot), and stay in registers between the sum and the norm; CHUNKS = 0 reads the stored sum again
+// (each thread its own stores).  The sum is normalised as stored, its squares added in f64 as
+// lm_gemm_rms_norm adds them.  Instructions bound it for 16-bit rows (f64 square root and division
+// in every thread took 62 us at 16384 x 2048, rsqrt 52) and HBM for f32 rows.
 template <int DT, bool VEC, int T, int CHUNKS>
-__global__ void __launch_bounds__(kThreads)
-    add_rms_norm_mx_kernel(const typename Elem<DT>::T* hidden, const void* delta, int delta_f32, const float* __restrict__ weight, int64_t rows,
-                           int64_t cols, float eps, typename Elem<DT>::T* sum, __nv_bfloat16* __restrict__ out_bf16, int format,
+__global__ void __launch_bounds__(T)
+    add_rms_norm_mx_kernel(const typename Elem<DT>::T* hidden, const void* delta, int delta_f32, const float* __restrict__ weight, int64_t cols,
+                           double inv_cols, double eps, typename Elem<DT>::T* sum, __nv_bfloat16* __restrict__ out_bf16, int format,
                            uint8_t* __restrict__ data, int64_t data_pitch, uint8_t* __restrict__ scales, int64_t scale_pitch) {
-    __shared__ double red[kWarps];
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreads / T) + threadIdx.x / T;
-    if (row >= rows) return;
-    const int64_t first = threadIdx.x % T * 8, end = scale_pitch * kMxBlock;
+    const int64_t row = blockIdx.x, first = threadIdx.x * 8, end = scale_pitch * kMxBlock;
     hidden += row * cols, sum += row * cols, data += row * data_pitch, scales += row * scale_pitch;
     if (delta != nullptr) delta = static_cast<const uint8_t*>(delta) + row * cols * (delta_f32 ? 4 : 2);
     if (out_bf16 != nullptr) out_bf16 += row * cols;
     double s = 0.0;
     if constexpr (CHUNKS > 0) {
-        float v[CHUNKS][8];
+        float v[CHUNKS][8], d[CHUNKS][8];
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) s += add_store<DT, VEC>(hidden, delta, delta_f32 != 0, first + c * T * 8, cols, sum, v[c]);
-        const float inverse = static_cast<float>(1.0 / sqrt(row_sum<T>(s, red) / static_cast<double>(cols) + static_cast<double>(eps)));
+        for (int c = 0; c < CHUNKS; ++c) load_pair<DT, VEC>(hidden, delta, delta_f32 != 0, first + c * T * 8, cols, v[c], d[c]);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) s += add_store<DT, VEC>(v[c], d[c], delta != nullptr, first + c * T * 8, cols, sum);
+        const float inverse = static_cast<float>(rsqrt(block_sum<T>(s) * inv_cols + eps));
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c)
             if (first + c * T * 8 < end) put_norm<VEC>(v[c], inverse, weight, first + c * T * 8, cols, out_bf16, format, data, data_pitch, scales);
     } else {
-        float v[8];
-        for (int64_t col = first; col < cols; col += T * 8) s += add_store<DT, VEC>(hidden, delta, delta_f32 != 0, col, cols, sum, v);
-        const float inverse = static_cast<float>(1.0 / sqrt(row_sum<T>(s, red) / static_cast<double>(cols) + static_cast<double>(eps)));
+        float v[8], d[8];
+        for (int64_t col = first; col < cols; col += T * 8) {
+            load_pair<DT, VEC>(hidden, delta, delta_f32 != 0, col, cols, v, d);
+            s += add_store<DT, VEC>(v, d, delta != nullptr, col, cols, sum);
+        }
+        const float inverse = static_cast<float>(rsqrt(block_sum<T>(s) * inv_cols + eps));
         for (int64_t col = first; col < end; col += T * 8) {
             load_cols<DT, VEC>(sum, col, cols, v);
             put_norm<VEC>(v, inverse, weight, col, cols, out_bf16, format, data, data_pitch, scales);
@@ -207,14 +237,9 @@ __global__ void __launch_bounds__(kThreads)
 
 bool is_mx_format(int32_t format) { return format == LM_MX_E2M1 || format == LM_MX_E4M3; }
 
-// Calls f with the segments' number in the type that holds it, and the grid for them.
-template <class F>
-lm_status with_segments(int64_t segments, F&& f) {
-    const int64_t each = kWarps * kFlight, blocks = (segments + each - 1) / each;
-    if (blocks > INT32_MAX) return context_free_fail(LM_ERR_UNSUPPORTED, "an MX matrix of more than 2^44 columns in all");
-    if (segments <= INT32_MAX - each) f(static_cast<uint32_t>(segments), static_cast<unsigned>(blocks));
-    else f(segments, static_cast<unsigned>(blocks));
-    return context_free_finish(cudaGetLastError());
+// Blocks of kWarps rows by kFlight segments.
+dim3 grid_for(int64_t rows, int64_t cols) {
+    return dim3(static_cast<unsigned>((rows + kWarps - 1) / kWarps), static_cast<unsigned>((cols + kFlight * kSegCols - 1) / (kFlight * kSegCols)));
 }
 
 }  // namespace
@@ -238,20 +263,18 @@ lm_status lm_mx_quantize(const void* values, int32_t dtype, int64_t rows, int64_
     if (rows == 0 || cols == 0) return LM_OK;
     if (values == nullptr || data == nullptr || scales == nullptr || !aligned(values, elem_size(dtype)) || !aligned(data, 32) || !aligned(scales, 16))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_mx_quantize: data must be 32-byte aligned and scales 16-byte aligned");
-    const int segs = static_cast<int>(mx_scale_pitch(cols) / 8);
     const bool vec = aligned(values, 16) && row_stride * elem_size(dtype) % 16 == 0;
-    const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return with_segments(rows * segs, [&](auto total, unsigned grid) {
-        with_dtype(dtype, [&](auto dt) {
-            with_format(format, [&](auto fmt) {
-                with_bool(vec, [&](auto v) {
-                    using T = typename Elem<decltype(dt)::value>::T;
-                    mx_quantize_kernel<decltype(dt)::value, decltype(fmt)::value, decltype(v)::value><<<grid, kThreads, 0, s>>>(
-                        static_cast<const T*>(values), total, cols, row_stride, segs, data, mx_data_pitch(format, cols), scales);
-                });
+    const dim3 grid = grid_for(rows, mx_scale_pitch(cols) * kMxBlock);
+    with_dtype(dtype, [&](auto dt) {
+        with_format(format, [&](auto fmt) {
+            with_bool(vec, [&](auto v) {
+                using T = typename Elem<decltype(dt)::value>::T;
+                mx_quantize_kernel<decltype(dt)::value, decltype(fmt)::value, decltype(v)::value><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+                    static_cast<const T*>(values), rows, cols, row_stride, data, mx_data_pitch(format, cols), scales, mx_scale_pitch(cols));
             });
         });
     });
+    return context_free_finish(cudaGetLastError());
 }
 
 lm_status lm_mx_dequantize(const uint8_t* data, const uint8_t* scales, int32_t format, int64_t rows, int64_t cols, void* values,
@@ -263,20 +286,18 @@ lm_status lm_mx_dequantize(const uint8_t* data, const uint8_t* scales, int32_t f
     if (rows == 0 || cols == 0) return LM_OK;
     if (values == nullptr || data == nullptr || scales == nullptr || !aligned(values, elem_size(dtype)) || !aligned(data, 32) || !aligned(scales, 16))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_mx_dequantize: data must be 32-byte aligned and scales 16-byte aligned");
-    const int segs = static_cast<int>((cols + kSegCols - 1) / kSegCols);
     const bool vec = aligned(values, 16) && row_stride * elem_size(dtype) % 16 == 0;
-    const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return with_segments(rows * segs, [&](auto total, unsigned grid) {
-        with_dtype(dtype, [&](auto dt) {
-            with_format(format, [&](auto fmt) {
-                with_bool(vec, [&](auto v) {
-                    using T = typename Elem<decltype(dt)::value>::T;
-                    mx_dequantize_kernel<decltype(dt)::value, decltype(fmt)::value, decltype(v)::value><<<grid, kThreads, 0, s>>>(
-                        data, mx_data_pitch(format, cols), scales, mx_scale_pitch(cols), total, cols, segs, static_cast<T*>(values), row_stride);
-                });
+    const dim3 grid = grid_for(rows, cols);
+    with_dtype(dtype, [&](auto dt) {
+        with_format(format, [&](auto fmt) {
+            with_bool(vec, [&](auto v) {
+                using T = typename Elem<decltype(dt)::value>::T;
+                mx_dequantize_kernel<decltype(dt)::value, decltype(fmt)::value, decltype(v)::value><<<grid, kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+                    data, mx_data_pitch(format, cols), scales, mx_scale_pitch(cols), rows, cols, static_cast<T*>(values), row_stride);
             });
         });
     });
+    return context_free_finish(cudaGetLastError());
 }
 
 lm_status lm_gemm_add_rms_norm_mx(const void* hidden, int32_t dtype, const void* delta, int32_t delta_dtype, const float* weight,
@@ -296,24 +317,22 @@ lm_status lm_gemm_add_rms_norm_mx(const void* hidden, int32_t dtype, const void*
     // Rows of a whole number of 16-byte words, all starting on one: eight columns a load.
     const bool vec = count % 8 == 0 && aligned(hidden, 16) && aligned(sum, 16) && aligned(delta, 16) && aligned(out_bf16, 16) && aligned(weight, 16);
     const int64_t wide = mx_scale_pitch(count) * kMxBlock;
-    // A warp a row while its registers hold the row and there are enough rows to fill the GPU (16384
-    // rows of 2048 bf16: MEASURE); else a CTA a row, for the latency of few rows and for wide ones.
-    const bool warp_rows = wide <= 2048 && rows >= 148 * 4 * kWarps;
     with_bool(dtype == LM_DTYPE_F32, [&](auto hf) {
         with_bool(vec, [&](auto v) {
             constexpr int DT = decltype(hf)::value ? LM_DTYPE_F32 : LM_DTYPE_BF16;
             constexpr bool VEC = decltype(v)::value;
             using T = typename Elem<DT>::T;
             const auto go = [&](auto threads, auto chunks) {
-                constexpr int per = kThreads / decltype(threads)::value;
-                add_rms_norm_mx_kernel<DT, VEC, decltype(threads)::value, decltype(chunks)::value><<<static_cast<unsigned>((rows + per - 1) / per), kThreads, 0, s>>>(
-                    static_cast<const T*>(hidden), delta, delta_dtype == LM_DTYPE_F32, weight, rows, count, epsilon, static_cast<T*>(sum),
+                constexpr int N = decltype(threads)::value;
+                add_rms_norm_mx_kernel<DT, VEC, N, decltype(chunks)::value><<<static_cast<unsigned>(rows), N, 0, s>>>(
+                    static_cast<const T*>(hidden), delta, delta_dtype == LM_DTYPE_F32, weight, count, 1.0 / static_cast<double>(count), epsilon, static_cast<T*>(sum),
                     reinterpret_cast<__nv_bfloat16*>(out_bf16), format, data, mx_data_pitch(format, count), scales, mx_scale_pitch(count));
             };
-            if (warp_rows) go(std::integral_constant<int, 32>{}, std::integral_constant<int, 8>{});
-            else if (wide <= 2048) go(std::integral_constant<int, kThreads>{}, std::integral_constant<int, 1>{});
-            else if (wide <= 8192) go(std::integral_constant<int, kThreads>{}, std::integral_constant<int, 4>{});
-            else go(std::integral_constant<int, kThreads>{}, std::integral_constant<int, 0>{});
+            const auto one = std::integral_constant<int, 1>{};
+            if (wide <= 2048) go(std::integral_constant<int, 256>{}, one);
+            else if (wide <= 4096) go(std::integral_constant<int, 512>{}, one);
+            else if (wide <= 8192) go(std::integral_constant<int, 1024>{}, one);
+            else go(std::integral_constant<int, 1024>{}, std::integral_constant<int, 0>{});
         });
     });
     return context_free_finish(cudaGetLastError());

@@ -16,7 +16,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWarps = kPlanThreads / 32;
 constexpr int kPlanMaxExperts = 1024;
-constexpr int kPlanMaxCluster = 8;
+constexpr int kPlanCluster = 8;
 constexpr int kRowThreads = 256;
 constexpr int kRowWarps = kRowThreads / 32;
 
@@ -27,12 +27,24 @@ __device__ __forceinline__ int ld_cluster(const int* v, uint32_t rank) {
     return r;
 }
 
-// One cluster.  Each warp takes a contiguous run of pairs and counts them per expert in its own
-// histogram; a scan over (expert, CTA, warp) turns the counts into first rows; a second pass over
-// the run hands the rows out in order.  The CTAs read one another's totals through distributed
+// The lanes of the warp that hold the same x: a vote for each bit.  (With __match_any_sync each
+// pass took half as long again.)
+__device__ __forceinline__ unsigned same_lanes(unsigned x, int bits) {
+    unsigned m = 0xffffffffu;
+    for (int b = 0; b < bits; ++b) {
+        const bool set = x >> b & 1u;
+        const unsigned v = __ballot_sync(0xffffffffu, set);
+        m &= set ? v : ~v;
+    }
+    return m;
+}
+
+// One cluster.  Each warp takes a contiguous run of pairs, counts them per expert in its own
+// histogram and notes each pair's place there; a scan over (expert, CTA, warp) turns the counts into
+// first rows, which are added to the places.  The CTAs read one another's totals through distributed
 // shared memory, so that no workspace is needed and two plans at once share nothing.
 __global__ void __launch_bounds__(kPlanThreads)
-    sort_plan_kernel(const int32_t* __restrict__ idx, int64_t pairs, int experts, int32_t* __restrict__ offsets, int32_t* __restrict__ at) {
+    sort_plan_kernel(const int32_t* __restrict__ idx, int pairs, int experts, int32_t* __restrict__ offsets, int32_t* __restrict__ at) {
     extern __shared__ int hist[];  // [warp][expert], then this CTA's totals [expert]
     __shared__ int scan[kPlanWarps];
     int* totals = hist + kPlanWarps * experts;
@@ -40,21 +52,25 @@ __global__ void __launch_bounds__(kPlanThreads)
     const int rank = static_cast<int>(cluster_ctarank()), ctas = static_cast<int>(gridDim.x);
     for (int i = threadIdx.x; i < kPlanWarps * experts; i += kPlanThreads) hist[i] = 0;
     __syncthreads();
-    const int64_t groups = (pairs + 31) / 32, runs = static_cast<int64_t>(ctas) * kPlanWarps, run = static_cast<int64_t>(rank) * kPlanWarps + warp;
-    const int64_t g0 = groups * run / runs, g1 = groups * (run + 1) / runs;
+    const int groups = (pairs + 31) / 32, runs = ctas * kPlanWarps, run = rank * kPlanWarps + warp;
+    const int each = groups / runs, more = groups % runs;  // the first `more` runs take one group of 32 pairs more
+    const int p0 = (run * each + min(run, more)) * 32, p1 = min(pairs, p0 + (each + (run < more)) * 32);
     int* mine = hist + warp * experts;
-    const auto load = [&](int64_t g) {
-        const int64_t p = g * 32 + lane;
-        const int x = g < g1 && p < pairs ? idx[p] : -1;
-        return x < experts ? x : -1;
-    };
-    int x = load(g0), next = load(g0 + 1);
-    for (int64_t g = g0; g < g1; ++g) {
-        const int after = load(g + 2);
-        const unsigned same = __match_any_sync(0xffffffffu, x);
-        if (x >= 0 && __ffs(same) - 1 == lane) mine[x] += __popc(same);
+    const int bits = 32 - __clz(experts);
+    const unsigned none = static_cast<unsigned>(experts);  // a dropped pair's expert
+    // Counts the run and leaves in `at` each pair's place among its expert's pairs of this run.
+    unsigned next = p0 + lane < p1 ? static_cast<unsigned>(idx[p0 + lane]) : none;
+    for (int p = p0 + lane; p - lane < p1; p += 32) {
+        const unsigned x = min(next, none);
+        next = p + 32 < p1 ? static_cast<unsigned>(idx[p + 32]) : none;
+        const unsigned same = same_lanes(x, bits);
+        const unsigned below = same & ((1u << lane) - 1u);
+        int place = -1;
+        if (x != none) place = mine[x] + __popc(below);
         __syncwarp();
-        x = next, next = after;
+        if (x != none && below == 0) mine[x] = place + __popc(same);
+        __syncwarp();
+        if (p < p1) at[p] = place;
     }
     __syncthreads();
     // Thread e: its expert's total here and in the other CTAs, the exclusive scan over experts, and
@@ -108,17 +124,10 @@ __global__ void __launch_bounds__(kPlanThreads)
         }
     }
     __syncthreads();
-    x = load(g0), next = load(g0 + 1);
-    for (int64_t g = g0; g < g1; ++g) {
-        const int after = load(g + 2);
-        const int64_t p = g * 32 + lane;
-        const unsigned same = __match_any_sync(0xffffffffu, x);
-        const int row = x >= 0 ? mine[x] + __popc(same & ((1u << lane) - 1u)) : -1;
-        __syncwarp();
-        if (x >= 0 && __ffs(same) - 1 == lane) mine[x] += __popc(same);
-        __syncwarp();
-        if (p < pairs) at[p] = row;
-        x = next, next = after;
+#pragma unroll 4
+    for (int p = p0 + lane; p < p1; p += 32) {
+        const unsigned x = static_cast<unsigned>(idx[p]);
+        if (x < none) at[p] += mine[x];
     }
 }
 
@@ -151,124 +160,174 @@ __global__ void __launch_bounds__(kRowThreads)
     }
 }
 
-// V consecutive values of a row from column c on; V is 8 for rows of whole 16-byte words, else 1.
+// ── back, and the gradients ──────────────────────────────────────────────
+// V consecutive elements of a row: 8 for rows of whole 16-byte words, else 1.
 template <int DT, int V>
-__device__ __forceinline__ void load_row(const typename Elem<DT>::T* p, float (&v)[V]) {
-    if constexpr (V == 8) load8<DT>(p, v);
-    else v[0] = Elem<DT>::widen(*p);
-}
-template <int DT, int V>
-__device__ __forceinline__ void store_row(typename Elem<DT>::T* p, const float (&v)[V]) {
-    if constexpr (V == 8) store8<DT>(p, v);
-    else *p = Elem<DT>::narrow(v[0]);
-}
+struct Part {
+    Raw8<DT> r;
+    __device__ __forceinline__ void load(const typename Elem<DT>::T* p) { r.load(p); }
+    __device__ __forceinline__ void widen(float (&v)[V]) const { r.widen(v); }
+    static __device__ __forceinline__ void store(typename Elem<DT>::T* p, const float (&v)[V]) { store8<DT>(p, v); }
+};
+template <int DT>
+struct Part<DT, 1> {
+    typename Elem<DT>::T e;
+    __device__ __forceinline__ void load(const typename Elem<DT>::T* p) { e = *p; }
+    __device__ __forceinline__ void widen(float (&v)[1]) const { v[0] = Elem<DT>::widen(e); }
+    static __device__ __forceinline__ void store(typename Elem<DT>::T* p, const float (&v)[1]) { *p = Elem<DT>::narrow(v[0]); }
+};
 
 constexpr int kSlots = 4;  // rows whose loads are in flight together
+// and stretches of 32 V columns of each: what 80 registers a thread hold
+template <int DT, int V>
+constexpr int kStretches = V == 1 ? 4 : DT == LM_DTYPE_F32 ? 1 : 2;
 
-// A warp takes 32 V columns of a token: y = the sum over its slots in order, in f32, rounded once.
+// The next up to kSlots slots of a token that have a row: bits of `left`, in order.  A lane holds
+// the row and weight of slot j0 + lane.
+struct NextSlots {
+    int row[kSlots], slot[kSlots];
+    float weight[kSlots];
+    __device__ __forceinline__ void take(unsigned& left, int my_row, float my_weight) {
+#pragma unroll
+        for (int q = 0; q < kSlots; ++q) {
+            slot[q] = left != 0 ? __ffs(left) - 1 : -1;
+            left &= left - 1;
+            row[q] = __shfl_sync(0xffffffffu, my_row, slot[q] & 31);
+            weight[q] = __shfl_sync(0xffffffffu, my_weight, slot[q] & 31);
+        }
+    }
+};
+
+// A warp takes kStretches x 32 V columns of a token: y = the sum over its slots in order, in f32,
+// rounded once.
 template <int DT, int DY, int V>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 3)
     unsort_rows_kernel(const typename Elem<DT>::T* __restrict__ rows, int64_t n_rows, const int32_t* __restrict__ at,
                        const float* __restrict__ weights, int64_t tokens, int k, int64_t cols, int parts, typename Elem<DY>::T* __restrict__ y,
                        int accumulate) {
+    constexpr int U = kStretches<DT, V>;
     const int lane = threadIdx.x & 31;
     const int64_t w = static_cast<int64_t>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5), t = w / parts;
     if (t >= tokens) return;
-    const int64_t c = ((w - t * parts) * 32 + lane) * V;
-    const bool live = c < cols;
-    float s[V];
+    const int64_t c = ((w - t * parts) * (32 * U) + lane) * V;
+    float s[U][V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) s[i] = 0.0f;
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[u][i] = 0.0f;
     for (int j0 = 0; j0 < k; j0 += 32) {
-        const int my_row = j0 + lane < k ? at[t * k + j0 + lane] : -1;
+        int my_row = j0 + lane < k ? at[t * k + j0 + lane] : -1;
+        if (my_row >= n_rows) my_row = -1;
         const float my_weight = weights != nullptr && j0 + lane < k ? weights[t * k + j0 + lane] : 1.0f;
-        for (int j = 0; j < min(32, k - j0); j += kSlots) {
-            float v[kSlots][V];
-            bool has[kSlots];
+        for (unsigned left = __ballot_sync(0xffffffffu, my_row >= 0); left != 0;) {
+            NextSlots next;
+            next.take(left, my_row, my_weight);
+            Part<DT, V> v[kSlots][U];
+#pragma unroll
+            for (int q = 0; q < kSlots; ++q)
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    if (next.slot[q] >= 0 && c + u * 32 * V < cols) v[q][u].load(rows + next.row[q] * cols + c + u * 32 * V);
 #pragma unroll
             for (int q = 0; q < kSlots; ++q) {
-                const int r = __shfl_sync(0xffffffffu, my_row, (j + q) & 31);
-                has[q] = j + q < 32 && r >= 0 && r < n_rows && live;
-                if (has[q]) load_row<DT, V>(rows + r * cols + c, v[q]);
-            }
+                if (next.slot[q] < 0) break;
 #pragma unroll
-            for (int q = 0; q < kSlots; ++q) {
-                const float weight = __shfl_sync(0xffffffffu, my_weight, (j + q) & 31);
-                if (has[q]) {
+                for (int u = 0; u < U; ++u) {
+                    float f[V];
+                    v[q][u].widen(f);
 #pragma unroll
-                    for (int i = 0; i < V; ++i) s[i] = fmaf(weight, v[q][i], s[i]);
+                    for (int i = 0; i < V; ++i) s[u][i] = fmaf(next.weight[q], f[i], s[u][i]);
                 }
             }
         }
     }
-    if (!live) return;
-    typename Elem<DY>::T* dst = y + t * cols + c;
-    if (accumulate) {
-        float v[V];
-        load_row<DY, V>(dst, v);
 #pragma unroll
-        for (int i = 0; i < V; ++i) s[i] += v[i];
+    for (int u = 0; u < U; ++u) {
+        if (c + u * 32 * V >= cols) break;
+        typename Elem<DY>::T* dst = y + t * cols + c + u * 32 * V;
+        if (accumulate) {
+            Part<DY, V> old;
+            float f[V];
+            old.load(dst);
+            old.widen(f);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s[u][i] += f[i];
+        }
+        Part<DY, V>::store(dst, s[u]);
     }
-    store_row<DY, V>(dst, s);
 }
 
-// grad_rows[at] = w grad_y, grad_weights = <grad_y, rows[at]> (0 for a dropped pair).  W warps take
-// a token's columns in turns, kSlots slots at a time, and add their dot products at the end.
+// grad_rows[at] = w grad_y, grad_weights = <grad_y, rows[at]> (0 for a dropped pair).  W warps of a
+// CTA take a token, its columns in turns, and add their dot products in order at the end.
 template <int DT, int V, int W>
-__global__ void __launch_bounds__(kRowThreads)
+__global__ void __launch_bounds__(kRowThreads, 3)
     unsort_rows_backward_kernel(const typename Elem<DT>::T* __restrict__ grad_y, const typename Elem<DT>::T* rows, int64_t n_rows,
                                 const int32_t* __restrict__ at, const float* __restrict__ weights, int64_t tokens, int k, int64_t cols,
                                 typename Elem<DT>::T* grad_rows, float* __restrict__ grad_weights) {
-    __shared__ float red[kRowWarps][kSlots];
+    constexpr int U = kStretches<DT, V>;
+    __shared__ float red[kRowWarps][LM_SORT_MAX_TOP_K];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * (kRowWarps / W) + warp / W;
-    if (t >= tokens) return;
-    for (int j0 = 0; j0 < k; j0 += kSlots) {
-        int r[kSlots];
-        float weight[kSlots], dot[kSlots];
+    if (t < tokens) {
+        for (int j0 = 0; j0 < k; j0 += 32) {
+            int my_row = j0 + lane < k ? at[t * k + j0 + lane] : -1;
+            if (my_row >= n_rows) my_row = -1;
+            const float my_weight = j0 + lane < k ? weights[t * k + j0 + lane] : 0.0f;
+            red[warp][j0 + lane] = 0.0f;
+            __syncwarp();
+            for (unsigned left = __ballot_sync(0xffffffffu, my_row >= 0); left != 0;) {
+                NextSlots next;
+                next.take(left, my_row, my_weight);
+                float dot[kSlots];
 #pragma unroll
-        for (int q = 0; q < kSlots; ++q) {
-            r[q] = j0 + q < k ? at[t * k + j0 + q] : -1;
-            if (r[q] >= n_rows) r[q] = -1;
-            weight[q] = r[q] >= 0 ? weights[t * k + j0 + q] : 0.0f;
-            dot[q] = 0.0f;
-        }
-        for (int64_t c = (warp % W * 32 + lane) * V; c < cols; c += W * 32 * V) {
-            float g[V], v[kSlots][V];
-            load_row<DT, V>(grad_y + t * cols + c, g);
+                for (int q = 0; q < kSlots; ++q) dot[q] = 0.0f;
+                for (int64_t c = (warp % W * 32 * U + lane) * V; c < cols; c += W * 32 * U * V) {
+                    Part<DT, V> g[U], v[kSlots][U];
 #pragma unroll
-            for (int q = 0; q < kSlots; ++q)
-                if (r[q] >= 0) load_row<DT, V>(rows + r[q] * cols + c, v[q]);
+                    for (int u = 0; u < U; ++u)
+                        if (c + u * 32 * V < cols) g[u].load(grad_y + t * cols + c + u * 32 * V);
 #pragma unroll
-            for (int q = 0; q < kSlots; ++q) {
-                if (r[q] < 0) continue;
-                float out[V];
+                    for (int q = 0; q < kSlots; ++q)
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    dot[q] = fmaf(g[i], v[q][i], dot[q]);
-                    out[i] = weight[q] * g[i];
+                        for (int u = 0; u < U; ++u)
+                            if (next.slot[q] >= 0 && c + u * 32 * V < cols) v[q][u].load(rows + next.row[q] * cols + c + u * 32 * V);
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        if (c + u * 32 * V >= cols) break;
+                        float gf[V];
+                        g[u].widen(gf);
+#pragma unroll
+                        for (int q = 0; q < kSlots; ++q) {
+                            if (next.slot[q] < 0) break;
+                            float f[V], out[V];
+                            v[q][u].widen(f);
+#pragma unroll
+                            for (int i = 0; i < V; ++i) {
+                                dot[q] = fmaf(gf[i], f[i], dot[q]);
+                                out[i] = next.weight[q] * gf[i];
+                            }
+                            Part<DT, V>::store(grad_rows + next.row[q] * cols + c + u * 32 * V, out);
+                        }
+                    }
                 }
-                store_row<DT, V>(grad_rows + r[q] * cols + c, out);
+#pragma unroll
+                for (int q = 0; q < kSlots; ++q) {
+                    if (next.slot[q] < 0) break;
+                    for (int off = 16; off > 0; off >>= 1) dot[q] += __shfl_xor_sync(0xffffffffu, dot[q], off);
+                    if (lane == 0) red[warp][j0 + next.slot[q]] = dot[q];
+                }
             }
         }
+    }
+    __syncthreads();
+    const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (kRowWarps / W);
+    for (int i = threadIdx.x; i < kRowWarps / W * k; i += kRowThreads) {
+        const int token = i / k, j = i - token * k;
+        if (t0 + token >= tokens) break;
+        float s = 0.0f;
 #pragma unroll
-        for (int q = 0; q < kSlots; ++q)
-            for (int off = 16; off > 0; off >>= 1) dot[q] += __shfl_xor_sync(0xffffffffu, dot[q], off);
-        if constexpr (W > 1) {
-            if (lane == 0)
-                for (int q = 0; q < kSlots; ++q) red[warp][q] = dot[q];
-            __syncthreads();
-            if (threadIdx.x < kSlots && j0 + threadIdx.x < k) {
-                float s = 0.0f;
-                for (int i = 0; i < W; ++i) s += red[i][threadIdx.x];
-                grad_weights[t * k + j0 + threadIdx.x] = s;
-            }
-            __syncthreads();
-        } else {
-#pragma unroll
-            for (int q = 0; q < kSlots; ++q)
-                if (lane == q && j0 + q < k) grad_weights[t * k + j0 + q] = dot[q];
-        }
+        for (int w = 0; w < W; ++w) s += red[token * W + w][j];
+        grad_weights[(t0 + token) * k + j] = s;
     }
 }
 
@@ -298,10 +357,10 @@ lm_status lm_moe_sort_plan(const int32_t* topk_idx, int64_t tokens, int32_t top_
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_sort_plan: tokens x top_k beyond 2^31, top_k beyond 64 or experts beyond 1024");
     if (offsets == nullptr || !aligned(offsets, 4) || (tokens > 0 && (topk_idx == nullptr || at == nullptr || !aligned(topk_idx, 4) || !aligned(at, 4))))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_sort_plan: a null or misaligned pointer");
-    // A CTA for each 4096 pairs (four rounds of a warp's 32), up to a cluster of eight.
+    // A cluster's launch and its two barriers cost 1.4 us more than one CTA, which takes 0.7 us for each
+    // 1000 pairs (8000 pairs: one CTA 8.5 us, two 7.2, four 5.9, eight 5.2; 98304: 67 and 12.4).
     const int64_t pairs = tokens * top_k;
-    int ctas = 1;
-    while (ctas < kPlanMaxCluster && pairs > int64_t(4096) * ctas) ctas *= 2;
+    const int ctas = pairs <= 2048 ? 1 : kPlanCluster;
     const int smem = (kPlanWarps + 1) * experts * 4;
     if (smem > 40 * 1024)
         if (const cudaError_t e = cudaFuncSetAttribute(sort_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kPlanWarps + 1) * kPlanMaxExperts * 4);
@@ -318,7 +377,7 @@ lm_status lm_moe_sort_plan(const int32_t* topk_idx, int64_t tokens, int32_t top_
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     cfg.attrs = &cluster;
     cfg.numAttrs = 1;
-    return context_free_finish(cudaLaunchKernelEx(&cfg, sort_plan_kernel, topk_idx, pairs, static_cast<int>(experts), offsets, at));
+    return context_free_finish(cudaLaunchKernelEx(&cfg, sort_plan_kernel, topk_idx, static_cast<int>(pairs), static_cast<int>(experts), offsets, at));
 }
 
 lm_status lm_moe_sort_rows(const void* x, int64_t x_stride, const int32_t* at, int64_t tokens, int32_t top_k, int64_t row_bytes, void* rows,
@@ -355,21 +414,24 @@ lm_status lm_moe_unsort_rows(const void* rows, int32_t dtype, int64_t n_rows, co
         !aligned(weights, 4))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows: a null or misaligned pointer");
     const bool vec = cols % 8 == 0 && aligned(rows, 16) && aligned(y, 16);
-    return with_parts(tokens, (cols + (vec ? 255 : 31)) / (vec ? 256 : 32), [&](unsigned grid, int parts) {
-        with_dtype(dtype, [&](auto dt) {
-            with_bool(vec, [&](auto v) {
-                constexpr int DT = decltype(dt)::value, V = decltype(v)::value ? 8 : 1;
-                const auto go = [&](auto dy) {
-                    constexpr int DY = decltype(dy)::value;
+    lm_status st = LM_OK;
+    with_dtype(dtype, [&](auto dt) {
+        with_bool(vec, [&](auto v) {
+            constexpr int DT = decltype(dt)::value, V = decltype(v)::value ? 8 : 1;
+            constexpr int64_t each = 32 * V * kStretches<DT, V>;
+            const auto go = [&](auto dy) {
+                constexpr int DY = decltype(dy)::value;
+                st = with_parts(tokens, (cols + each - 1) / each, [&](unsigned grid, int parts) {
                     unsort_rows_kernel<DT, DY, V><<<grid, kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
                         static_cast<const typename Elem<DT>::T*>(rows), n_rows, at, weights, tokens, top_k, cols, parts, static_cast<typename Elem<DY>::T*>(y),
                         accumulate != 0);
-                };
-                if (y_dtype == LM_DTYPE_F32) go(std::integral_constant<int, LM_DTYPE_F32>{});
-                else go(dt);
-            });
+                });
+            };
+            if (y_dtype == LM_DTYPE_F32) go(std::integral_constant<int, LM_DTYPE_F32>{});
+            else go(dt);
         });
     });
+    return st;
 }
 
 lm_status lm_moe_unsort_rows_backward(const void* grad_y, const void* rows, int32_t dtype, int64_t n_rows, const int32_t* at, const float* weights,
@@ -383,17 +445,22 @@ lm_status lm_moe_unsort_rows_backward(const void* grad_y, const void* rows, int3
         !aligned(grad_weights, 4))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows_backward: a null or misaligned pointer");
     const bool vec = cols % 8 == 0 && aligned(grad_y, 16) && aligned(rows, 16) && aligned(grad_rows, 16);
-    // A warp a token when that fills the GPU, else all eight warps of a CTA.
-    const bool wide = tokens < 148 * 4 * kRowWarps;
     with_dtype(dtype, [&](auto dt) {
         with_bool(vec, [&](auto v) {
-            with_bool(wide, [&](auto wd) {
-                constexpr int DT = decltype(dt)::value, W = decltype(wd)::value ? kRowWarps : 1, per = kRowWarps / W;
-                using T = typename Elem<DT>::T;
-                unsort_rows_backward_kernel<DT, decltype(v)::value ? 8 : 1, W>
-                    <<<static_cast<unsigned>((tokens + per - 1) / per), kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-                        static_cast<const T*>(grad_y), static_cast<const T*>(rows), n_rows, at, weights, tokens, top_k, cols, static_cast<T*>(grad_rows), grad_weights);
-            });
+            constexpr int DT = decltype(dt)::value, V = decltype(v)::value ? 8 : 1;
+            using T = typename Elem<DT>::T;
+            const auto go = [&](auto warps) {
+                constexpr int W = decltype(warps)::value, per = kRowWarps / W;
+                unsort_rows_backward_kernel<DT, V, W><<<static_cast<unsigned>((tokens + per - 1) / per), kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+                    static_cast<const T*>(grad_y), static_cast<const T*>(rows), n_rows, at, weights, tokens, top_k, cols, static_cast<T*>(grad_rows), grad_weights);
+            };
+            // As many warps a token as its row has stretches for them (2048 bf16 columns, 16384 tokens:
+            // one warp 89 us, two 87, four 93, eight, half of them idle, 127; 1 token: 8.3, 5.6, 4.2).
+            const int64_t pieces = (cols + 32 * V * kStretches<DT, V> - 1) / (32 * V * kStretches<DT, V>);
+            if (pieces <= 1) go(std::integral_constant<int, 1>{});
+            else if (pieces <= 2) go(std::integral_constant<int, 2>{});
+            else if (pieces <= 4) go(std::integral_constant<int, 4>{});
+            else go(std::integral_constant<int, 8>{});
         });
     });
     return context_free_finish(cudaGetLastError());

@@ -180,11 +180,11 @@ def mx_matmul(x: MxTensor, w: MxTensor, offsets=None, dtype=torch.bfloat16, out=
     return out
 
 
-def mx_sync(device=None) -> None:
-    """lm_mx_sync: waits for the device's current stream and raises if a product gave up waiting."""
+def sync(device=None) -> None:
+    """lm_ops_sync: waits for the device's current stream and raises if a kernel gave up waiting."""
     device = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index or 0)
     with _on(device):
-        check(load().lm_mx_sync(_stream(device)))
+        check(load().lm_ops_sync(_stream(device)))
 
 
 def add_rms_norm(hidden, delta, weight, eps: float, fmt: str = "e4m3", bf16: bool = False, out=None):

@@ -242,7 +242,7 @@ def test_product_same_every_time():
     first = ops.mx_matmul(x, w, offsets, dtype=F32)
     for _ in range(5):
         same_bits(ops.mx_matmul(x, w, offsets, dtype=F32), first)
-    ops.mx_sync()  # nothing gave up waiting
+    ops.sync()  # nothing gave up waiting
 
 
 # ---------------------------------------------------------------- the residual norm
