@@ -9,8 +9,6 @@ argument that does not fit (before any launch) or ``LiteMindError`` with the lib
 """
 from __future__ import annotations
 
-from contextlib import nullcontext
-
 import torch
 
 from . import _lib
@@ -18,6 +16,13 @@ from ._lib import check, load
 
 _DTYPES = {torch.float32: _lib.LM_DTYPE_F32, torch.bfloat16: _lib.LM_DTYPE_BF16, torch.float16: _lib.LM_DTYPE_F16}
 _FORMATS = {"e2m1": _lib.LM_MX_E2M1, "e4m3": _lib.LM_MX_E4M3}
+_RESIDUAL = (torch.float32, torch.bfloat16)
+
+# The calls for a few rows take a few microseconds on the GPU, so what Python adds counts: messages
+# are made only when they are raised, outputs with new_empty (cheaper than torch.empty with a
+# device), and the stream's handle is taken without building a torch.cuda.Stream (2 us).
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _need(ok: bool, message: str) -> None:
@@ -25,54 +30,67 @@ def _need(ok: bool, message: str) -> None:
         raise ValueError(message)
 
 
-def _same_device(*tensors) -> torch.device:
-    """The one CUDA device that all the tensors (None left out) are on."""
-    device = None
-    for t in tensors:
-        if t is not None:
-            _need(t.is_cuda, "tensors must be on a CUDA device")
-            if device is None:
-                device = t.device
-            else:
-                _need(t.device == device, "all tensors must be on one device")
-    return device
+def _index(first, *others) -> int:
+    """The index of the one CUDA device that all the tensors (None left out) are on."""
+    index = first.get_device()
+    if index < 0:
+        raise ValueError("tensors must be on a CUDA device")
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError("all tensors must be on one device")
+    return index
 
 
-def _on(device: torch.device):
-    """Makes `device` current for a call, when it is not."""
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _call(fn, index: int, *args) -> None:
+    """fn(*args, stream) with the device current and its current stream."""
+    if torch.cuda.current_device() == index:
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        check(status)
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _matrix(t, name: str):
-    _need(t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]),
-          f"{name} must be a matrix with contiguous, non-overlapping rows")
-
-
-def _row_stride(t) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _row_stride(t, name: str) -> int:
+    """Elements from row to row of a matrix with contiguous rows that do not overlap."""
+    if t.dim() == 2:
+        rows, cols = t.shape
+        if rows <= 1 or cols == 0:
+            stride = cols
+        else:
+            stride = t.stride(0)
+        if (cols <= 1 or t.stride(1) == 1) and stride >= cols:
+            return stride
+    raise ValueError(f"{name} must be a matrix with contiguous, non-overlapping rows")
 
 
 def _dtype(t, name: str) -> int:
     code = _DTYPES.get(t.dtype)
-    _need(code is not None, f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if code is None:
+        raise ValueError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
     return code
 
 
 def _format(fmt: str) -> int:
     code = _FORMATS.get(fmt)
-    _need(code is not None, f"unknown MX format {fmt!r}: e2m1 or e4m3")
+    if code is None:
+        raise ValueError(f"unknown MX format {fmt!r}: e2m1 or e4m3")
     return code
+
+
+def _full(t, shape, dtype, message: str) -> None:
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(message)
 
 
 # ---------------------------------------------------------------- MX matrices
 
 
-def _pad(n: int, to: int) -> int:
-    return -(-n // to) * to
+def _pitches(cols: int, fmt: str) -> tuple:
+    """Bytes of one row of data and of scales (lm_mx_data_pitch, lm_mx_scale_pitch)."""
+    wide = -(-cols // 128) * 128
+    return (wide // 2 if fmt == "e2m1" else wide), -(-cols // 512) * 16
 
 
 class MxTensor:
@@ -90,18 +108,26 @@ class MxTensor:
         _format(fmt)
         _need(data.dtype == torch.uint8 and scales.dtype == torch.uint8 and data.is_contiguous() and scales.is_contiguous(),
               "data and scales must be contiguous uint8 tensors")
-        wide = _pad(cols, 128)
-        _need(data.dim() >= 2 and data.shape[:-1] == scales.shape[:-1] and data.shape[-1] == (wide // 2 if fmt == "e2m1" else wide)
-              and scales.shape[-1] == _pad(cols, 512) // 32, f"data and scales do not have the layout of {cols} {fmt} columns")
+        if data.dim() < 2 or data.shape[:-1] != scales.shape[:-1] or (data.shape[-1], scales.shape[-1]) != _pitches(cols, fmt):
+            raise ValueError(f"data and scales do not have the layout of {cols} {fmt} columns")
         self.data, self.scales, self.cols, self.fmt = data, scales, cols, fmt
 
     @classmethod
     def empty(cls, shape, fmt: str, device="cuda") -> "MxTensor":
         """An uninitialised one of the given [..., rows, cols]."""
-        *lead, cols = shape
-        wide = _pad(cols, 128)
-        return cls(torch.empty((*lead, wide // 2 if fmt == "e2m1" else wide), dtype=torch.uint8, device=device),
-                   torch.empty((*lead, _pad(cols, 512) // 32), dtype=torch.uint8, device=device), cols, fmt)
+        _format(fmt)
+        return cls._like(torch.empty(0, dtype=torch.uint8, device=device), shape, fmt)
+
+    @classmethod
+    def _like(cls, t, shape, fmt: str) -> "MxTensor":
+        """An uninitialised one on t's device."""
+        x = cls.__new__(cls)
+        *lead, x.cols = shape
+        x.fmt = fmt
+        data, scales = _pitches(x.cols, fmt)
+        x.data = t.new_empty((*lead, data), dtype=torch.uint8)
+        x.scales = x.data.new_empty((*lead, scales))
+        return x
 
     @property
     def shape(self) -> tuple:
@@ -119,37 +145,32 @@ class MxTensor:
 def mx_quantize(values, fmt: str, out: MxTensor | None = None) -> MxTensor:
     """lm_mx_quantize of a float32, bfloat16 or float16 [..., cols] tensor (more than two
     dimensions: contiguous)."""
-    code = _dtype(values, "values")
+    code, format_code = _dtype(values, "values"), _format(fmt)
     if values.dim() == 2:
-        _matrix(values, "values")
-        flat = values
+        rows, cols = values.shape
+        stride = _row_stride(values, "values")
     else:
         _need(values.dim() > 2 and values.is_contiguous(), "values must be a matrix, or contiguous with more dimensions")
-        flat = values.view(-1, values.shape[-1])
-    device = _same_device(values)
+        cols = stride = values.shape[-1]
+        rows = values.numel() // cols if cols else 0
     if out is None:
-        out = MxTensor.empty(values.shape, fmt, device)
+        index = _index(values)
+        out = MxTensor._like(values, values.shape, fmt)
     else:
         _need(out.shape == tuple(values.shape) and out.fmt == fmt, "out has another shape or format")
-        _same_device(values, out.data, out.scales)
-    with _on(device):
-        check(load().lm_mx_quantize(flat.data_ptr(), code, flat.shape[0], flat.shape[1], _row_stride(flat), _format(fmt),
-                                    out.data.data_ptr(), out.scales.data_ptr(), _stream(device)))
+        index = _index(values, out.data, out.scales)
+    _call(load().lm_mx_quantize, index, values.data_ptr(), code, rows, cols, stride, format_code, out.data.data_ptr(), out.scales.data_ptr())
     return out
 
 
 def mx_dequantize(x: MxTensor, dtype=torch.float32, out=None):
     """lm_mx_dequantize: the values that x stands for, as `dtype`."""
-    device = _same_device(x.data, x.scales)
+    index = _index(x.data, x.scales, out)
     if out is None:
-        out = torch.empty(x.shape, dtype=dtype, device=device)
+        out = x.data.new_empty(x.shape, dtype=dtype)
     else:
-        _need(tuple(out.shape) == x.shape and out.dtype == dtype and out.is_contiguous(), "out has another shape or type, or is not contiguous")
-        _same_device(x.data, out)
-    code = _dtype(out, "out")
-    with _on(device):
-        check(load().lm_mx_dequantize(x.data.data_ptr(), x.scales.data_ptr(), _FORMATS[x.fmt], x.rows, x.cols, out.data_ptr(), code, x.cols,
-                                      _stream(device)))
+        _full(out, x.shape, dtype, "out has another shape or type, or is not contiguous")
+    _call(load().lm_mx_dequantize, index, x.data.data_ptr(), x.scales.data_ptr(), _FORMATS[x.fmt], x.rows, x.cols, out.data_ptr(), _dtype(out, "out"), x.cols)
     return out
 
 
@@ -159,56 +180,52 @@ def mx_matmul(x: MxTensor, w: MxTensor, offsets=None, dtype=torch.bfloat16, out=
 
     offsets: int32 [groups + 1] on the device (SortPlan.offsets); None with one group (w may be
     [n, k] then).  Rows of no group keep what `out` held."""
-    _need(x.data.dim() == 2 and w.data.dim() in (2, 3) and w.fmt == "e2m1" and x.cols == w.cols,
-          "x must be [rows, k] and w 4-bit [groups, n, k] with the same k")
-    groups = w.data.shape[0] if w.data.dim() == 3 else 1
-    rows, n = x.data.shape[0], w.data.shape[-2]
-    device = _same_device(x.data, x.scales, w.data, w.scales, offsets, out)
+    wd = w.data.shape
+    _need(x.data.dim() == 2 and len(wd) in (2, 3) and w.fmt == "e2m1" and x.cols == w.cols, "x must be [rows, k] and w 4-bit [groups, n, k] with the same k")
+    groups = wd[0] if len(wd) == 3 else 1
+    rows, n = x.data.shape[0], wd[-2]
+    index = _index(x.data, x.scales, w.data, w.scales, offsets, out)
     if offsets is None:
         _need(groups == 1, "several groups need offsets")
     else:
         _need(offsets.dtype == torch.int32 and offsets.is_contiguous() and offsets.numel() == groups + 1, "offsets must be int32 [groups + 1]")
     if out is None:
-        out = torch.empty((rows, n), dtype=dtype, device=device)
+        out = x.data.new_empty((rows, n), dtype=dtype)
+        stride = n
     else:
         _need(tuple(out.shape) == (rows, n) and out.dtype == dtype, "out has another shape or type")
-        _matrix(out, "out")
-    code = _dtype(out, "out")
-    with _on(device):
-        check(load().lm_mx_matmul(x.data.data_ptr(), x.scales.data_ptr(), _FORMATS[x.fmt], rows, w.data.data_ptr(), w.scales.data_ptr(), groups, n,
-                                  x.cols, None if offsets is None else offsets.data_ptr(), out.data_ptr(), code, _row_stride(out), _stream(device)))
+        stride = _row_stride(out, "out")
+    _call(load().lm_mx_matmul, index, x.data.data_ptr(), x.scales.data_ptr(), _FORMATS[x.fmt], rows, w.data.data_ptr(), w.scales.data_ptr(), groups, n, x.cols,
+          None if offsets is None else offsets.data_ptr(), out.data_ptr(), _dtype(out, "out"), stride)
     return out
 
 
 def sync(device=None) -> None:
     """lm_ops_sync: waits for the device's current stream and raises if a kernel gave up waiting."""
-    device = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device(device).index or 0)
-    with _on(device):
-        check(load().lm_ops_sync(_stream(device)))
+    index = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    _call(load().lm_ops_sync, index)
 
 
 def add_rms_norm(hidden, delta, weight, eps: float, fmt: str = "e4m3", bf16: bool = False, out=None):
     """lm_gemm_add_rms_norm_mx: (hidden + delta, its RMS norm as an MxTensor, the norm in bfloat16
     or None).  hidden and delta (may be None): contiguous float32 or bfloat16 [rows, cols]; weight
     float32 [cols].  The sum has hidden's type and goes to `out`, which may be hidden itself."""
-    _need(hidden.dim() == 2 and hidden.is_contiguous() and hidden.dtype in (torch.float32, torch.bfloat16), "hidden must be contiguous float32 or bfloat16 [rows, cols]")
-    if delta is not None:
-        _need(delta.shape == hidden.shape and delta.is_contiguous() and delta.dtype in (torch.float32, torch.bfloat16),
-              "delta must be contiguous float32 or bfloat16 of hidden's shape")
+    _need(hidden.dim() == 2 and hidden.is_contiguous() and hidden.dtype in _RESIDUAL, "hidden must be contiguous float32 or bfloat16 [rows, cols]")
+    _need(delta is None or (delta.shape == hidden.shape and delta.is_contiguous() and delta.dtype in _RESIDUAL),
+          "delta must be contiguous float32 or bfloat16 of hidden's shape")
     rows, cols = hidden.shape
-    _need(weight.dtype == torch.float32 and weight.is_contiguous() and tuple(weight.shape) == (cols,), "weight must be contiguous float32 [cols]")
-    device = _same_device(hidden, delta, weight, out)
+    _full(weight, (cols,), torch.float32, "weight must be contiguous float32 [cols]")
+    format_code = _format(fmt)
+    index = _index(hidden, delta, weight, out)
     if out is None:
         out = torch.empty_like(hidden)
     else:
-        _need(out.shape == hidden.shape and out.dtype == hidden.dtype and out.is_contiguous(), "out must be contiguous, of hidden's shape and type")
-    q = MxTensor.empty((rows, cols), fmt, device)
-    plain = torch.empty((rows, cols), dtype=torch.bfloat16, device=device) if bf16 else None
-    with _on(device):
-        check(load().lm_gemm_add_rms_norm_mx(hidden.data_ptr(), _DTYPES[hidden.dtype], None if delta is None else delta.data_ptr(),
-                                             _DTYPES[hidden.dtype if delta is None else delta.dtype], weight.data_ptr(), rows, cols, eps,
-                                             out.data_ptr(), None if plain is None else plain.data_ptr(), _FORMATS[fmt], q.data.data_ptr(),
-                                             q.scales.data_ptr(), _stream(device)))
+        _full(out, hidden.shape, hidden.dtype, "out must be contiguous, of hidden's shape and type")
+    q = MxTensor._like(hidden, (rows, cols), fmt)
+    plain = hidden.new_empty((rows, cols), dtype=torch.bfloat16) if bf16 else None
+    _call(load().lm_gemm_add_rms_norm_mx, index, hidden.data_ptr(), _DTYPES[hidden.dtype], None if delta is None else delta.data_ptr(),
+          _DTYPES[hidden.dtype if delta is None else delta.dtype], weight.data_ptr(), rows, cols, eps, out.data_ptr(),
+          None if plain is None else plain.data_ptr(), format_code, q.data.data_ptr(), q.scales.data_ptr())
     return out, q, plain
 
 
@@ -234,29 +251,28 @@ def sort_plan(topk_idx, experts: int) -> SortPlan:
     """lm_moe_sort_plan of int32 [tokens, top_k] expert indices (outside [0, experts): dropped)."""
     _need(topk_idx.dtype == torch.int32 and topk_idx.dim() == 2 and topk_idx.is_contiguous(), "topk_idx must be contiguous int32 [tokens, top_k]")
     _need(0 < experts <= 1024, "experts must be in 1 .. 1024")
-    device = _same_device(topk_idx)
-    offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
-    at = torch.empty_like(topk_idx)
-    with _on(device):
-        check(load().lm_moe_sort_plan(topk_idx.data_ptr(), topk_idx.shape[0], topk_idx.shape[1], experts, offsets.data_ptr(), at.data_ptr(),
-                                      _stream(device)))
-    return SortPlan(offsets, at)
+    index = _index(topk_idx)
+    plan = SortPlan.__new__(SortPlan)
+    plan.offsets, plan.at = topk_idx.new_empty((experts + 1,)), torch.empty_like(topk_idx)
+    tokens, k = topk_idx.shape
+    _call(load().lm_moe_sort_plan, index, topk_idx.data_ptr(), tokens, k, experts, plan.offsets.data_ptr(), plan.at.data_ptr())
+    return plan
 
 
 def _sort(x, plan: SortPlan, out):
-    _matrix(x, "x")
-    tokens, k = plan.at.shape
+    x_stride = _row_stride(x, "x")
+    (tokens, k), cols = plan.at.shape, x.shape[1]
     _need(x.shape[0] == tokens, "x must have a row for each token of the plan")
     if out is None:
-        out = torch.empty((tokens * k, x.shape[1]), dtype=x.dtype, device=x.device)
+        index = _index(x, plan.at)
+        out = x.new_empty((tokens * k, cols))
+        out_stride = cols
     else:
-        _matrix(out, "out")
-        _need(out.dtype == x.dtype and out.shape[1] == x.shape[1], "out must have x's type and columns")
-    device = _same_device(x, plan.at, out)
+        out_stride = _row_stride(out, "out")
+        _need(out.dtype == x.dtype and out.shape[1] == cols, "out must have x's type and columns")
+        index = _index(x, plan.at, out)
     z = x.element_size()
-    with _on(device):
-        check(load().lm_moe_sort_rows(x.data_ptr(), _row_stride(x) * z, plan.at.data_ptr(), tokens, k, x.shape[1] * z, out.data_ptr(),
-                                      _row_stride(out) * z, out.shape[0], _stream(device)))
+    _call(load().lm_moe_sort_rows, index, x.data_ptr(), x_stride * z, plan.at.data_ptr(), tokens, k, cols * z, out.data_ptr(), out_stride * z, out.shape[0])
     return out
 
 
@@ -276,20 +292,20 @@ def unsort_rows(rows, plan: SortPlan, weights=None, out=None, dtype=None, accumu
     accumulate adds to `out`."""
     _need(rows.dim() == 2 and rows.is_contiguous(), "rows must be a contiguous matrix")
     code = _dtype(rows, "rows")
-    tokens, k = plan.at.shape
+    (tokens, k), (n_rows, cols) = plan.at.shape, rows.shape
     if weights is not None:
-        _need(weights.dtype == torch.float32 and weights.shape == plan.at.shape and weights.is_contiguous(), "weights must be contiguous float32 [tokens, top_k]")
+        _full(weights, (tokens, k), torch.float32, "weights must be contiguous float32 [tokens, top_k]")
     if out is None:
         _need(not accumulate, "accumulate needs out")
-        out = torch.empty((tokens, rows.shape[1]), dtype=dtype or rows.dtype, device=rows.device)
+        _need(dtype is None or dtype in (rows.dtype, torch.float32), "the result has rows' type or float32")
+        index = _index(rows, plan.at, weights)
+        out = rows.new_empty((tokens, cols), dtype=dtype)
     else:
-        _need(tuple(out.shape) == (tokens, rows.shape[1]) and out.is_contiguous() and (dtype is None or out.dtype == dtype),
-              "out must be contiguous [tokens, cols] of the given type")
-    _need(out.dtype in (rows.dtype, torch.float32), "the result has rows' type or float32")
-    device = _same_device(rows, plan.at, weights, out)
-    with _on(device):
-        check(load().lm_moe_unsort_rows(rows.data_ptr(), code, rows.shape[0], plan.at.data_ptr(), None if weights is None else weights.data_ptr(), tokens, k,
-                                        rows.shape[1], out.data_ptr(), _DTYPES[out.dtype], int(accumulate), _stream(device)))
+        _need(out.dtype in (rows.dtype, torch.float32), "the result has rows' type or float32")
+        _full(out, (tokens, cols), dtype or out.dtype, "out must be contiguous [tokens, cols] of the given type")
+        index = _index(rows, plan.at, weights, out)
+    _call(load().lm_moe_unsort_rows, index, rows.data_ptr(), code, n_rows, plan.at.data_ptr(), None if weights is None else weights.data_ptr(), tokens, k, cols,
+          out.data_ptr(), _DTYPES[out.dtype], int(accumulate))
     return out
 
 
@@ -302,19 +318,17 @@ def unsort_rows_backward(grad_y, rows, plan: SortPlan, weights, out=None):
     """lm_moe_unsort_rows_backward: (grad_rows, grad_weights) of unsort_rows with weights.
     grad_rows goes to `out` (which may be rows itself); rows of no pair keep what it held
     (uninitialised without it)."""
-    _need(rows.dim() == 2 and rows.is_contiguous() and grad_y.dim() == 2 and grad_y.is_contiguous() and grad_y.dtype == rows.dtype,
-          "grad_y and rows must be contiguous matrices of one type")
+    _need(rows.dim() == 2 and rows.is_contiguous(), "rows must be a contiguous matrix")
     code = _dtype(rows, "rows")
-    tokens, k = plan.at.shape
-    _need(tuple(grad_y.shape) == (tokens, rows.shape[1]), "grad_y must be [tokens, cols]")
-    _need(weights.dtype == torch.float32 and weights.shape == plan.at.shape and weights.is_contiguous(), "weights must be contiguous float32 [tokens, top_k]")
+    (tokens, k), (n_rows, cols) = plan.at.shape, rows.shape
+    _full(grad_y, (tokens, cols), rows.dtype, "grad_y must be contiguous [tokens, cols] of rows' type")
+    _full(weights, (tokens, k), torch.float32, "weights must be contiguous float32 [tokens, top_k]")
+    index = _index(grad_y, rows, plan.at, weights, out)
     if out is None:
         out = torch.empty_like(rows)
     else:
-        _need(out.shape == rows.shape and out.dtype == rows.dtype and out.is_contiguous(), "out must be contiguous, of rows' shape and type")
-    device = _same_device(grad_y, rows, plan.at, weights, out)
+        _full(out, rows.shape, rows.dtype, "out must be contiguous, of rows' shape and type")
     grad_weights = torch.empty_like(weights)
-    with _on(device):
-        check(load().lm_moe_unsort_rows_backward(grad_y.data_ptr(), rows.data_ptr(), code, rows.shape[0], plan.at.data_ptr(), weights.data_ptr(), tokens, k,
-                                                 rows.shape[1], out.data_ptr(), grad_weights.data_ptr(), _stream(device)))
+    _call(load().lm_moe_unsort_rows_backward, index, grad_y.data_ptr(), rows.data_ptr(), code, n_rows, plan.at.data_ptr(), weights.data_ptr(), tokens, k, cols,
+          out.data_ptr(), grad_weights.data_ptr())
     return out, grad_weights
