@@ -4,16 +4,19 @@
 //   D[128 rows of W_g, BN rows of X] = W_g X^T,   out[r, n] = D[n, r]
 //
 // The weights are the MMA's M side, so that a few rows of X cost a narrow N instead of a padded M.
-// One persistent CTA an SM walks the tiles (group, BN rows of X, 128 rows of W).  Its warps:
-//   0      TMA producer: a ring of stages of 256 columns.  4-bit codes travel packed (half a byte a
-//          column from HBM and L2) and are spread by the TMA into the MMA's padded form.
-//   1      MMA issuer: eight block-scaled MMAs of 32 columns a stage
-//   2      scale producer: 32 bytes of each row, the scales of 1024 columns, to shared memory by TMA,
-//          up to three such chunks ahead
+// One persistent CTA an SM walks the tiles (group, BN rows of X, 128 rows of W); for many rows a
+// group, pairs of CTAs walk tiles of 256 rows of W together, each bringing its half of both operands
+// (so that L2 delivers 47 bytes a cycle to an SM at the full rate of the MMA, not 92: it can 57).
+// A CTA's warps:
+//   0      TMA producer: a ring of stages of one or two boxes of 128 columns.  4-bit codes travel
+//          packed (half a byte a column from HBM and L2); the TMA spreads them into the MMA's padded form.
+//   1      MMA issuer (of the pair's first CTA): four block-scaled MMAs of 32 columns a box
+//   2      scale producer: the scales of a chunk of boxes, to shared memory by TMA, ahead of the codes
 //   4-7    scales from shared memory to TMEM, each warp to its own quadrant
-//   8-11   epilogue: TMEM to registers to out, rounded once; double buffered against the MMA
+//   8-15   epilogue: TMEM to registers to out, rounded once; two warps a quadrant share the rows of X
 // A stage costs the issuer about 400 cycles of waits, descriptors and commits whatever its width,
-// and four MMAs take 200 (N = 16) to 256 (N = 128): hence eight of them a stage.
+// and the four MMAs of a box take 200 (N = 16) to 256 (N = 128) or, in a pair, 512 (N = 256): hence
+// two boxes a stage where they are short.
 // Every wait is bounded (ptx.cuh): a pipeline that stalls records a status for lm_ops_sync.
 #include "moe_internal.h"
 #include "mx_block.cuh"
@@ -25,27 +28,33 @@ namespace lm {
 namespace {
 
 constexpr int kBlockM = 128;
-constexpr int kBoxCols = 128;       // columns of a TMA box: one 128-byte row of the swizzled tiles
-constexpr int kStageBoxes = 2;
-constexpr int kChunkBoxes = 8;      // a chunk of scales: 32 bytes a row
-constexpr int kChunkBytes = 32;
-constexpr int kChunks = 3;
-constexpr int kThreads = 384;
+constexpr int kBoxCols = 128;  // columns of a TMA box: one 128-byte row of the swizzled tiles
+constexpr int kThreads = 512;
 constexpr int kSms = 148;
+constexpr int kMaxSplit = 4;
 constexpr int kABoxBytes = kBlockM * kBoxCols;
 
-template <int BN>
+template <int BN, bool PAIR>
 struct Cfg {
-    static constexpr int kBBoxBytes = BN * kBoxCols;
+    static constexpr int kCtas = PAIR ? 2 : 1;
+    static constexpr int kBRows = BN / kCtas;  // rows of X that a CTA brings
+    static constexpr int kBBoxBytes = kBRows * kBoxCols;
+    static constexpr int kStageBoxes = 2;
     static constexpr int kStageBytes = kStageBoxes * (kABoxBytes + kBBoxBytes);
+    static constexpr int kBoxSf = 8;  // TMEM columns of a box's scales: 4 of W's, 4 of X's
+    // A chunk of scales: 4 bytes of a row for each box.  The TMEM that the two accumulators leave
+    // holds four chunks or more.
+    static constexpr int kChunkBoxes = 8, kChunkBytes = 4 * kChunkBoxes, kChunks = 3;
+    static constexpr int kSfCols = kChunkBoxes * kBoxSf, kSfGroups = 4;
     static constexpr int kScaleBytes = (kBlockM + BN) * kChunkBytes;
-    static constexpr int kFit = (216 * 1024 - kChunks * kScaleBytes) / kStageBytes;
-    static constexpr int kStages = kFit > 8 ? 8 : kFit;
+    static constexpr int kStagesFit = (216 * 1024 - kChunks * kScaleBytes) / kStageBytes;
+    static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
     static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kChunks * kScaleBytes;
-    static constexpr int kSfCols = kChunkBoxes * (4 + 4);  // TMEM columns of a chunk: per box 4 of W's scales, 4 of X's
-    static constexpr int kSfGroups = (512 - 2 * BN) / kSfCols;
-    static_assert(BN % 16 == 0 && BN >= 16 && BN <= 128, "N of an M = 128 MMA, two accumulators");
-    static_assert(kStages >= 3 && kSfGroups >= 2, "rings");
+    static_assert(BN % 16 == 0 && BN >= 16 && 2 * BN + kSfGroups * kSfCols <= 512 && (!PAIR || BN % 32 == 0), "N of the MMA");
+    static_assert(kBBoxBytes % 1024 == 0 || !PAIR, "swizzled tiles start on 1024 bytes");
+    // Stages of one round of the issuer: two where a box's MMAs are short and the ring is long.
+    static constexpr int kRound = kStages >= 5 ? 2 : 1;
+    static_assert(kStages >= 3 && kChunkBoxes % (kRound * kStageBoxes) == 0, "rings");
 };
 
 struct Args {
@@ -54,8 +63,10 @@ struct Args {
     int64_t out_stride;
     int rows, groups, n;
     int k_boxes;
+    int split;  // CTAs (a cluster) that share a tile's boxes; more than 1: a cluster has one tile
     int x_four_bit;
     int out_dtype;
+    int out_pairs;  // 16-bit elements n, n + 1 (n even) lie on 4-byte boundaries
     int* status;
 };
 
@@ -102,11 +113,11 @@ __device__ void cut_groups(const Args& a, int* cut, int* tiles) {
 
 struct Tile {
     int group, row0, rows;  // rows of X: row0 .. row0 + rows - 1
-    int n0;                 // first row of W_g
+    int n0;                 // first row of W_g for this CTA
 };
 
-template <int BN>
-__device__ __forceinline__ Tile tile_at(const Args& a, const int* cut, const int* tiles, int t, int m_blocks) {
+template <int BN, bool PAIR>
+__device__ __forceinline__ Tile tile_at(const Args& a, const int* cut, const int* tiles, int t, int m_blocks, int rank) {
     const int ct = t / m_blocks;
     int lo = 0, hi = a.groups;  // tiles[lo] <= ct < tiles[hi]
     while (hi - lo > 1) {
@@ -117,34 +128,80 @@ __device__ __forceinline__ Tile tile_at(const Args& a, const int* cut, const int
     r.group = lo;
     r.row0 = cut[lo] + (ct - tiles[lo]) * BN;
     r.rows = min(BN, cut[lo + 1] - r.row0);
-    r.n0 = (t - ct * m_blocks) * kBlockM;
+    r.n0 = (t - ct * m_blocks) * kBlockM * Cfg<BN, PAIR>::kCtas + rank * kBlockM;
     return r;
 }
 
-template <int DT>
-__device__ __forceinline__ void store_columns(void* out, int64_t at, int64_t stride, int cols, const uint32_t (&v)[16]) {
-    typename Elem<DT>::T* p = static_cast<typename Elem<DT>::T*>(out) + at;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (i < cols) p[i * stride] = Elem<DT>::narrow(__uint_as_float(v[i]));
+// The MMA's N for a tile of `rows` rows of X: no wider than they need.
+template <bool PAIR>
+__device__ __forceinline__ int mma_n(int rows) {
+    return PAIR ? (rows + 31) & ~31 : (rows + 15) & ~15;
 }
 
-template <int BN>
+// Columns v[0 .. 31] of the accumulator (this lane's n) to rows of out from `p` on, `rows` of them.
+// 16-bit types: neighbouring lanes swap values, and each stores two n of every second row.
+template <int DT>
+__device__ __forceinline__ void store_columns(typename Elem<DT>::T* p, int64_t stride, int rows, bool n_ok, bool pairs, const uint32_t (&v)[32]) {
+    if constexpr (DT != LM_DTYPE_F32) {
+        if (pairs) {
+            const int odd = threadIdx.x & 1;
+            uint32_t* q = reinterpret_cast<uint32_t*>(p - odd + odd * stride);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
+                const typename Elem<DT>::T e[2] = {Elem<DT>::narrow(__uint_as_float(odd ? got : v[j])), Elem<DT>::narrow(__uint_as_float(odd ? v[j + 1] : got))};
+                uint32_t w;
+                memcpy(&w, e, 4);
+                if (j + odd < rows) *q = w;
+                q += stride;  // two rows of 16-bit elements
+            }
+            return;
+        }
+    }
+    if (!n_ok) return;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+        if (j < rows) *p = Elem<DT>::narrow(__uint_as_float(v[j]));
+        p += stride;
+    }
+}
+
+template <int BN, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     mx_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                      const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_xs, const Args a) {
-    using C = Cfg<BN>;
-    constexpr int S = C::kStages, G = C::kSfGroups;
+    using C = Cfg<BN, PAIR>;
+    constexpr int S = C::kStages, G = C::kSfGroups, B = C::kStageBoxes;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ int s_cut[LM_MX_MAX_GROUPS + 1], s_tiles[LM_MX_MAX_GROUPS + 1];
-    __shared__ uint64_t full[S], empty[S], chunk_full[kChunks], chunk_empty[kChunks], sf_full[G], sf_empty[G], tmem_full[2], tmem_empty[2], drain;
+    // In a pair `full`, `sf_full` and `tmem_empty` are the first CTA's, whose warp 1 issues the MMAs;
+    // the MMAs' commits arrive in both CTAs.
+    __shared__ uint64_t full[S], empty[S], chunk_full[C::kChunks], chunk_empty[C::kChunks], sf_full[G], sf_empty[G], tmem_full[2], tmem_empty[2], drain;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
     uint8_t* smem_a = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* smem_b = smem_a + S * kStageBoxes * kABoxBytes;
-    uint8_t* smem_s = smem_b + S * kStageBoxes * C::kBBoxBytes;  // chunks: 128 rows of W's scales, then BN of X's
+    uint8_t* smem_b = smem_a + S * B * kABoxBytes;
+    uint8_t* smem_s = smem_b + S * B * C::kBBoxBytes;  // chunks: 128 rows of W's scales, then BN of X's
+    float* partial = reinterpret_cast<float*>(smem_a);  // with a split: the ring is idle when its only tile is done
     volatile int* abort_flag = &s_abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;
+    const int split = PAIR ? 1 : a.split, part = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+    const int ctas = C::kCtas * split, first = blockIdx.x / ctas, step = gridDim.x / ctas;
+    // This CTA's boxes, from a multiple of four: 16 bytes of scales.
+    const int quads = (a.k_boxes + 3) / 4, box0 = quads * part / split * 4, boxes = min(a.k_boxes, quads * (part + 1) / split * 4) - box0;
+
+    const auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+        return mbar_wait(bar, parity, abort_flag, a.status, code);
+    };
+    const auto commit = [&](uint64_t* bar) {
+        if constexpr (PAIR) umma_commit_both(bar);
+        else umma_commit(bar);
+    };
+    const auto arrive_first = [&](uint64_t* bar) {  // on the first CTA's barrier
+        if constexpr (PAIR) mbar_arrive_cluster(mapa_shared(smem_u32(bar), 0));
+        else mbar_arrive(bar);
+    };
 
     if (warp == 0 && lane == 0) {
         tma_prefetch_desc(&map_w);
@@ -152,16 +209,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_prefetch_desc(&map_ws);
         tma_prefetch_desc(&map_xs);
         for (int i = 0; i < S; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-        for (int i = 0; i < kChunks; ++i) mbar_init(&chunk_full[i], 1), mbar_init(&chunk_empty[i], 4);
-        for (int i = 0; i < G; ++i) mbar_init(&sf_full[i], 4), mbar_init(&sf_empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&tmem_full[i], 1), mbar_init(&tmem_empty[i], 4);
+        for (int i = 0; i < C::kChunks; ++i) mbar_init(&chunk_full[i], 1), mbar_init(&chunk_empty[i], 4);
+        for (int i = 0; i < G; ++i) mbar_init(&sf_full[i], 4 * C::kCtas), mbar_init(&sf_empty[i], 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&tmem_full[i], 1), mbar_init(&tmem_empty[i], 8 * C::kCtas);
         mbar_init(&drain, 1);
         s_abort = 0;
         fence_mbar_init();
     }
+    __syncwarp();
+    if constexpr (PAIR) cluster_sync();  // both CTAs' barriers exist before either signals the other's
     if (warp == 1) {
-        tmem_alloc(&s_tmem, 512);
-        tmem_relinquish();
+        if constexpr (PAIR) {
+            tmem_alloc_pair(&s_tmem, 512);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(&s_tmem, 512);
+            tmem_relinquish();
+        }
     }
     if (warp == 2) cut_groups<BN>(a, s_cut, s_tiles);
     tc_fence_before();
@@ -169,28 +233,40 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = s_tmem;
     const uint32_t tmem_sf = tmem + 2 * BN;
-    const int m_blocks = (a.n + kBlockM - 1) / kBlockM;
+    const int m_blocks = (a.n + kBlockM * C::kCtas - 1) / (kBlockM * C::kCtas);
     const int total = s_tiles[a.groups] * m_blocks;
 
     // In the issuing warps all lanes walk the loop and an elected one issues, so that descriptors and
     // addresses stay in uniform registers (under `if (lane == 0)` a stage took twice as long).
     if (warp == 0) {
         const uint32_t box_bytes = kABoxBytes / 2 + (a.x_four_bit ? C::kBBoxBytes / 2 : C::kBBoxBytes);
+        // Narrow tiles are for groups of few rows, whose weights are read once: they leave L2 first
+        // (128 tokens over 64 experts: 43.8 -> 41.8 us; with 128 rows a tile it cost 7%).
+        const uint64_t once = policy_evict_first();
         int stage = 0;
         uint32_t phase = 0, issued = 0, issued_phase = 0;
         bool ok = true;
-        for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
-            const Tile tile = tile_at<BN>(a, s_cut, s_tiles, t, m_blocks);
+        for (int t = first; ok && t < total; t += step) {
+            const Tile tile = tile_at<BN, PAIR>(a, s_cut, s_tiles, t, m_blocks, rank);
             const int w_row = tile.group * a.n + tile.n0;
-            for (int b = 0; b < a.k_boxes; b += kStageBoxes) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, abort_flag, a.status, kDevTimeoutProducer));
+            const int x_row = tile.row0 + rank * mma_n<PAIR>(tile.rows) / 2;
+            for (int b = 0; b < boxes; b += B) {
+                ok = __all_sync(0xffffffffu, wait(&empty[stage], phase ^ 1u, kDevTimeoutProducer));
                 if (!ok) break;
                 if (elect_one()) {
-                    const int boxes = min(kStageBoxes, a.k_boxes - b);
-                    mbar_arrive_expect_tx(&full[stage], boxes * box_bytes);
-                    for (int i = 0; i < boxes; ++i) {
-                        tma_load_2d(smem_a + (stage * kStageBoxes + i) * kABoxBytes, &map_w, &full[stage], (b + i) * kBoxCols, w_row);
-                        tma_load_2d(smem_b + (stage * kStageBoxes + i) * C::kBBoxBytes, &map_x, &full[stage], (b + i) * kBoxCols, tile.row0);
+                    const int n_boxes = min(B, boxes - b);
+                    if (rank == 0) mbar_arrive_expect_tx(&full[stage], C::kCtas * n_boxes * box_bytes);
+                    for (int i = 0; i < n_boxes; ++i) {
+                        uint8_t *da = smem_a + (stage * B + i) * kABoxBytes, *db = smem_b + (stage * B + i) * C::kBBoxBytes;
+                        if constexpr (PAIR) {
+                            const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
+                            tma_load_2d_pair(da, &map_w, bar, (box0 + b + i) * kBoxCols, w_row);
+                            tma_load_2d_pair(db, &map_x, bar, (box0 + b + i) * kBoxCols, x_row);
+                        } else {
+                            if constexpr (BN <= 64) tma_load_2d_hint(da, &map_w, &full[stage], (box0 + b + i) * kBoxCols, w_row, once);
+                            else tma_load_2d(da, &map_w, &full[stage], (box0 + b + i) * kBoxCols, w_row);
+                            tma_load_2d(db, &map_x, &full[stage], (box0 + b + i) * kBoxCols, x_row);
+                        }
                     }
                 }
                 __syncwarp();
@@ -199,57 +275,81 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (++stage == S) stage = 0, phase ^= 1u;
             }
         }
-        if (!ok)  // copies in flight land before the CTA's shared memory is given up
+        if (!ok && rank == 0)  // copies in flight land before shared memory is given up
             for (int i = 0; i < S; ++i)
                 if (issued & (1u << i)) mbar_wait_drain(&full[i], (issued_phase >> i) & 1u, 100000000ull);
-    } else if (warp == 1) {
+    } else if (warp == 1 && rank == 0) {
         int stage = 0, sg = 0, acc = 0;
         uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
-        bool ok = true, any = false, seen = false;
+        bool ok = true, any = false, seen = false, sf_seen = false;
         const uint32_t format = (a.x_four_bit ? kUmmaE2M1 : kUmmaE4M3) << 10;
         const uint64_t desc_a = umma_desc_sw128(smem_u32(smem_a)), desc_b = umma_desc_sw128(smem_u32(smem_b));
-        for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&tmem_empty[acc], acc_phase ^ 1u, abort_flag, a.status, kDevTimeoutMma));
+        constexpr int U = C::kRound;
+        const auto after = [](int st, int by) { return st + by >= S ? st + by - S : st + by; };
+        for (int t = first; ok && t < total; t += step) {
+            int width = BN;  // a pair's MMAs are no wider than the tile's rows need; one CTA's take 50 cycles at least
+            if constexpr (PAIR) width = mma_n<PAIR>(tile_at<BN, PAIR>(a, s_cut, s_tiles, t, m_blocks, rank).rows);
+            const uint32_t shape = format | static_cast<uint32_t>(width >> 3) << 17;
+            ok = __all_sync(0xffffffffu, wait(&tmem_empty[acc], acc_phase ^ 1u, kDevTimeoutMma));
             const uint32_t d = tmem + acc * BN;
-            for (int b = 0; ok && b < a.k_boxes; b += kStageBoxes) {
-                if (b % kChunkBoxes == 0) ok = mbar_wait(&sf_full[sg], sf_phase, abort_flag, a.status, kDevTimeoutMma);
-                if (!seen) ok = ok && mbar_wait(&full[stage], phase, abort_flag, a.status, kDevTimeoutMma);
-                if (b % kChunkBoxes == 0 || !seen) ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
+            for (int b = 0; ok && b < boxes; b += U * B) {
+                const int stages = min(U, (boxes - b + B - 1) / B);
+                const bool sf_begin = b % C::kChunkBoxes == 0;
+                if ((sf_begin && !sf_seen) || !seen) {
+                    ok = !sf_begin || sf_seen || wait(&sf_full[sg], sf_phase, kDevTimeoutMma);
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (u < stages) ok = ok && wait(&full[after(stage, u)], phase ^ (stage + u >= S), kDevTimeoutMma);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                }
                 tc_fence_after();
-                const int next = stage + 1 == S ? 0 : stage + 1;
-                // A look at the next stage while the tensor cores still work: even the wait for a
+                const bool last = b + stages * B >= boxes;
+                const bool sf_end = last || (b + stages * B) % C::kChunkBoxes == 0;
+                const int next = after(stage, stages), sg_next = sg + 1 == G ? 0 : sg + 1;
+                const uint32_t next_phase = phase ^ (stage + stages >= S);
+                // A look at the next round while the tensor cores still work: even the wait for a
                 // complete barrier costs as much as an MMA.
-                const bool look = mbar_test(&full[next], phase ^ (next == 0));
-                const bool last = b + kStageBoxes >= a.k_boxes;
-                const bool sf_end = last || (b + kStageBoxes) % kChunkBoxes == 0;
+                bool look = true;
+#pragma unroll
+                for (int u = 0; u < U; ++u) look = look && mbar_test(&full[after(next, u)], next_phase ^ (next + u >= S));
+                const bool sf_look = sf_end && mbar_test(&sf_full[sg_next], sf_phase ^ (sg_next == 0));
                 if (elect_one()) {
 #pragma unroll
-                    for (int i = 0; i < kStageBoxes; ++i) {
-                        if (b + i < a.k_boxes) {
-                            const uint64_t da = desc_a + static_cast<uint32_t>((stage * kStageBoxes + i) * (kABoxBytes >> 4));
-                            const uint64_t db = desc_b + static_cast<uint32_t>((stage * kStageBoxes + i) * (C::kBBoxBytes >> 4));
-                            const uint32_t sf = tmem_sf + sg * C::kSfCols + (b % kChunkBoxes + i) * 8;
+                    for (int u = 0; u < U; ++u) {
+                        if (u >= stages) break;
+                        const int st = after(stage, u);
 #pragma unroll
-                            for (int kk = 0; kk < 4; ++kk)  // 32 columns are 32 bytes, 2 in the descriptor's units
-                                umma_mx(d, da + 2 * kk, db + 2 * kk, umma_idesc_mx(kUmmaE2M1, 0, kBlockM, BN, kk) | format, sf, sf + 4,
-                                        b != 0 || i != 0 || kk != 0);
+                        for (int i = 0; i < B; ++i) {
+                            const int box = u * B + i;
+                            if (b + box < boxes) {
+                                const uint64_t da = desc_a + static_cast<uint32_t>((st * B + i) * (kABoxBytes >> 4));
+                                const uint64_t db = desc_b + static_cast<uint32_t>((st * B + i) * (C::kBBoxBytes >> 4));
+                                const uint32_t sf = tmem_sf + sg * C::kSfCols + (b % C::kChunkBoxes + box) * C::kBoxSf;
+#pragma unroll
+                                for (int kk = 0; kk < 4; ++kk) {  // 32 columns are 32 bytes, 2 in the descriptor's units
+                                    const uint32_t idesc = umma_idesc_mx(kUmmaE2M1, 0, kBlockM * C::kCtas, 0, kk) | shape;
+                                    const uint32_t add = b != 0 || box != 0 || kk != 0;
+                                    if constexpr (PAIR) umma_mx_pair(d, da + 2 * kk, db + 2 * kk, idesc, sf, sf + 4, add);
+                                    else umma_mx(d, da + 2 * kk, db + 2 * kk, idesc, sf, sf + 4, add);
+                                }
+                            }
                         }
+                        commit(&empty[st]);
                     }
-                    umma_commit(&empty[stage]);
-                    if (sf_end) umma_commit(&sf_empty[sg]);
-                    if (last) umma_commit(&tmem_full[acc]);
+                    if (sf_end) commit(&sf_empty[sg]);
+                    if (last) commit(&tmem_full[acc]);
                 }
                 __syncwarp();
                 any = true;
                 seen = __all_sync(0xffffffffu, look);
-                phase ^= next == 0, stage = next;
-                if (sf_end && ++sg == G) sg = 0, sf_phase ^= 1u;
+                phase = next_phase, stage = next;
+                if (sf_end) sf_seen = __all_sync(0xffffffffu, sf_look), sf_phase ^= sg_next == 0, sg = sg_next;
             }
             if (++acc == 2) acc = 0, acc_phase ^= 1u;
         }
         if (!ok && any) {  // the MMAs issued so far end before TMEM is released
-            if (elect_one()) umma_commit(&drain);
+            if (elect_one()) commit(&drain);
             __syncwarp();
             mbar_wait_drain(&drain, 0, 100000000ull);
         }
@@ -257,25 +357,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         int chunk = 0;
         uint32_t phase = 0, issued = 0, issued_phase = 0;
         bool ok = true;
-        for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
-            const Tile tile = tile_at<BN>(a, s_cut, s_tiles, t, m_blocks);
-            for (int b = 0; b < a.k_boxes; b += kChunkBoxes) {
+        for (int t = first; ok && t < total; t += step) {
+            const Tile tile = tile_at<BN, PAIR>(a, s_cut, s_tiles, t, m_blocks, rank);
+            for (int b = 0; b < boxes; b += C::kChunkBoxes) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&chunk_empty[chunk], phase ^ 1u, abort_flag, a.status, kDevTimeoutProducer));
                 if (!ok) break;
                 if (elect_one()) {
                     uint8_t* dst = smem_s + chunk * C::kScaleBytes;
                     mbar_arrive_expect_tx(&chunk_full[chunk], C::kScaleBytes);
-                    tma_load_2d(dst, &map_ws, &chunk_full[chunk], b / kChunkBoxes * kChunkBytes, tile.group * a.n + tile.n0);
-                    tma_load_2d(dst + kBlockM * kChunkBytes, &map_xs, &chunk_full[chunk], b / kChunkBoxes * kChunkBytes, tile.row0);
+                    tma_load_2d(dst, &map_ws, &chunk_full[chunk], (box0 + b) * 4, tile.group * a.n + tile.n0);
+                    tma_load_2d(dst + kBlockM * C::kChunkBytes, &map_xs, &chunk_full[chunk], (box0 + b) * 4, tile.row0);
                 }
                 __syncwarp();
                 issued |= 1u << chunk;
                 issued_phase = (issued_phase & ~(1u << chunk)) | (phase << chunk);
-                if (++chunk == kChunks) chunk = 0, phase ^= 1u;
+                if (++chunk == C::kChunks) chunk = 0, phase ^= 1u;
             }
         }
         if (!ok)
-            for (int i = 0; i < kChunks; ++i)
+            for (int i = 0; i < C::kChunks; ++i)
                 if (issued & (1u << i)) mbar_wait_drain(&chunk_full[i], (issued_phase >> i) & 1u, 100000000ull);
     } else if (warp >= 4 && warp < 8) {
         const uint32_t quad = static_cast<uint32_t>(warp & 3) * 32u << 16;
@@ -283,23 +383,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         int sg = 0, chunk = 0;
         uint32_t phase = 0, chunk_phase = 0;
         bool ok = true;
-        for (int t = blockIdx.x; ok && t < total; t += gridDim.x) {
-            for (int b = 0; ok && b < a.k_boxes; b += kChunkBoxes) {
+        for (int t = first; ok && t < total; t += step) {
+            for (int b = 0; b < boxes; b += C::kChunkBoxes) {
                 // Every lane waits for what it reads; a lane that gave up takes its warp along.
                 ok = mbar_wait(&chunk_full[chunk], chunk_phase, abort_flag, a.status, kDevTimeoutProducer);
-                ok = ok && mbar_wait(&sf_empty[sg], phase ^ 1u, abort_flag, a.status, kDevTimeoutProducer);
-                ok = __all_sync(0xffffffffu, ok);
+                ok = __all_sync(0xffffffffu, ok && wait(&sf_empty[sg], phase ^ 1u, kDevTimeoutProducer));
                 if (!ok) break;
                 tc_fence_after();
-                const uint8_t* src = smem_s + chunk * C::kScaleBytes + lane * kChunkBytes;
+                const uint8_t* src = smem_s + chunk * C::kScaleBytes + lane * C::kChunkBytes;
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {  // 8 bytes of a row are the scales of two boxes: 16 columns of TMEM
+                for (int h = 0; h < C::kChunkBoxes / 2; ++h) {  // 8 bytes of a row are its scales in two boxes
                     uint32_t r[16];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(src + 32 * c * kChunkBytes + 8 * h);
+                        const uint2 w = *reinterpret_cast<const uint2*>(src + 32 * c * C::kChunkBytes + 8 * h);
                         uint2 x = make_uint2(0u, 0u);
-                        if (c < kXRows && (BN >= 32 || lane < BN)) x = *reinterpret_cast<const uint2*>(src + (kBlockM + 32 * c) * kChunkBytes + 8 * h);
+                        if (c < kXRows && (BN >= 32 || lane < BN)) x = *reinterpret_cast<const uint2*>(src + (kBlockM + 32 * c) * C::kChunkBytes + 8 * h);
                         r[c] = w.x, r[8 + c] = w.y, r[4 + c] = x.x, r[12 + c] = x.y;
                     }
                     tmem_st16(tmem_sf + quad + sg * C::kSfCols + 16 * h, r);
@@ -308,48 +407,88 @@ __global__ void __launch_bounds__(kThreads, 1)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(&sf_full[sg]);
+                    arrive_first(&sf_full[sg]);
                     mbar_arrive(&chunk_empty[chunk]);
                 }
                 if (++sg == G) sg = 0, phase ^= 1u;
-                if (++chunk == kChunks) chunk = 0, chunk_phase ^= 1u;
+                if (++chunk == C::kChunks) chunk = 0, chunk_phase ^= 1u;
             }
         }
     } else if (warp >= 8) {
-        const int quad = warp & 3;
+        const int quad = warp & 3, half = (warp - 8) >> 2;
+        constexpr int kHalf = BN >= 64 ? BN / 2 : BN;  // a warp's rows of X; few: the first four warps take all
         int acc = 0;
         uint32_t acc_phase = 0;
-        for (int t = blockIdx.x; t < total; t += gridDim.x) {
-            const Tile tile = tile_at<BN>(a, s_cut, s_tiles, t, m_blocks);
+        for (int t = first; t < total; t += step) {
+            const Tile tile = tile_at<BN, PAIR>(a, s_cut, s_tiles, t, m_blocks, rank);
             int go = 1;
-            if (lane == 0) go = mbar_wait(&tmem_full[acc], acc_phase, abort_flag, a.status, kDevTimeoutEpilogue);
+            if (lane == 0) go = wait(&tmem_full[acc], acc_phase, kDevTimeoutEpilogue);
             if (__shfl_sync(0xffffffffu, go, 0) == 0) break;
             tc_fence_after();
-            const int n = tile.n0 + quad * 32 + lane;
+            const int n_warp = tile.n0 + quad * 32, n = n_warp + lane;
             const uint32_t src = tmem + acc * BN + (static_cast<uint32_t>(quad * 32) << 16);
-            for (int c0 = 0; c0 < tile.rows; c0 += 16) {
-                uint32_t v[16];
-                tmem_ld16(src + c0, v);
+            const bool pairs = a.out_pairs != 0 && n_warp + 32 <= a.n;
+            const int c_first = half * kHalf, c_end = min(tile.rows, c_first + kHalf);
+            for (int c0 = c_first; c0 < c_end; c0 += 32) {
+                uint32_t v[32];
+                tmem_ld16(src + c0, *reinterpret_cast<uint32_t(*)[16]>(v));
+                if constexpr (kHalf >= 32) tmem_ld16(src + c0 + 16, *reinterpret_cast<uint32_t(*)[16]>(v + 16));
                 tmem_ld_wait();
-                if (n < a.n) {
-                    const int64_t at = (static_cast<int64_t>(tile.row0) + c0) * a.out_stride + n;
-                    const int cols = tile.rows - c0;
-                    if (a.out_dtype == LM_DTYPE_F32) store_columns<LM_DTYPE_F32>(a.out, at, a.out_stride, cols, v);
-                    else if (a.out_dtype == LM_DTYPE_BF16) store_columns<LM_DTYPE_BF16>(a.out, at, a.out_stride, cols, v);
-                    else store_columns<LM_DTYPE_F16>(a.out, at, a.out_stride, cols, v);
+                if (split > 1) {  // this part's sums, for the cluster to add
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (c0 + j < c_end) partial[(c0 + j) * kBlockM + quad * 32 + lane] = __uint_as_float(v[j]);
+                    continue;
                 }
+                const int64_t at = (static_cast<int64_t>(tile.row0) + c0) * a.out_stride + n;
+                const int rows = c_end - c0;
+                if (a.out_dtype == LM_DTYPE_F32) store_columns<LM_DTYPE_F32>(static_cast<float*>(a.out) + at, a.out_stride, rows, n < a.n, pairs, v);
+                else if (a.out_dtype == LM_DTYPE_BF16) store_columns<LM_DTYPE_BF16>(static_cast<__nv_bfloat16*>(a.out) + at, a.out_stride, rows, n < a.n, pairs, v);
+                else store_columns<LM_DTYPE_F16>(static_cast<__half*>(a.out) + at, a.out_stride, rows, n < a.n, pairs, v);
                 __syncwarp();
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&tmem_empty[acc]);
+            if (lane == 0) arrive_first(&tmem_empty[acc]);
             if (++acc == 2) acc = 0, acc_phase ^= 1u;
+        }
+    }
+    if constexpr (!PAIR) {
+        if (split > 1) {
+            // The parts' sums, added in the parts' order, each CTA its share of the tile's elements.
+            __syncthreads();
+            cluster_sync();
+            if (first < total) {
+                const Tile tile = tile_at<BN, PAIR>(a, s_cut, s_tiles, first, m_blocks, rank);
+                for (int i = part * kThreads + threadIdx.x; i < tile.rows * kBlockM; i += split * kThreads) {
+                    float sum = 0.0f, v[kMaxSplit];
+#pragma unroll
+                    for (int p = 0; p < kMaxSplit; ++p)
+                        if (p < split) v[p] = ld_cluster_f32(mapa_shared(smem_u32(partial + i), p));
+#pragma unroll
+                    for (int p = 0; p < kMaxSplit; ++p)
+                        if (p < split) sum += v[p];
+                    const int n = tile.n0 + i % kBlockM;
+                    const int64_t at = (static_cast<int64_t>(tile.row0) + i / kBlockM) * a.out_stride + n;
+                    if (n < a.n) {
+                        if (a.out_dtype == LM_DTYPE_F32) static_cast<float*>(a.out)[at] = sum;
+                        else if (a.out_dtype == LM_DTYPE_BF16) static_cast<__nv_bfloat16*>(a.out)[at] = Elem<LM_DTYPE_BF16>::narrow(sum);
+                        else static_cast<__half*>(a.out)[at] = Elem<LM_DTYPE_F16>::narrow(sum);
+                    }
+                }
+            }
+            __syncwarp();
+            cluster_sync();  // no CTA leaves while another reads its sums
         }
     }
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();  // neither CTA leaves while the other may signal it or use its memory
     tc_fence_after();
-    if (warp == 1) tmem_dealloc(tmem, 512);
+    if (warp == 1) {
+        if constexpr (PAIR) tmem_dealloc_pair(tmem, 512);
+        else tmem_dealloc(tmem, 512);
+    }
 }
 
 struct Matrix {
@@ -359,22 +498,33 @@ struct Matrix {
     int64_t rows;
 };
 
-template <int BN>
+template <int BN, bool PAIR>
 lm_status launch(const Matrix& w, const Matrix& x, int64_t k, const Args& a, int64_t tiles, cudaStream_t stream) {
-    using C = Cfg<BN>;
+    using C = Cfg<BN, PAIR>;
     CUtensorMap map_w, map_x, map_ws, map_xs;
     std::string error;
     const uint64_t cols = static_cast<uint64_t>(mx_padded_cols(k)), pitch = static_cast<uint64_t>(mx_scale_pitch(k));
-    const auto encode = [&](const Matrix& m, uint32_t box, CUtensorMap* codes, CUtensorMap* scales) {
+    const auto encode = [&](const Matrix& m, uint32_t box, uint32_t scale_box, CUtensorMap* codes, CUtensorMap* scales) {
         return encode_tensor_map_mx(codes, m.codes, m.four_bit, static_cast<uint64_t>(m.rows), cols, box, error) &&
-               encode_tensor_map_mx_scales(scales, m.scales, static_cast<uint64_t>(m.rows), pitch, box, kChunkBytes, error);
+               encode_tensor_map_mx_scales(scales, m.scales, static_cast<uint64_t>(m.rows), pitch, scale_box, C::kChunkBytes, error);
     };
-    if (!encode(w, kBlockM, &map_w, &map_ws) || !encode(x, BN, &map_x, &map_xs)) return context_free_fail(LM_ERR_CUDA, error.c_str());
-    if (const cudaError_t e = cudaFuncSetAttribute(mx_matmul_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes); e != cudaSuccess)
-        return context_free_finish(e);
-    mx_matmul_kernel<BN><<<static_cast<unsigned>(std::min<int64_t>(tiles, kSms)), kThreads, C::kSmemBytes, stream>>>(map_w, map_x, map_ws, map_xs,
-                                                                                                                          a);
-    return context_free_finish(cudaGetLastError());
+    if (!encode(w, kBlockM, kBlockM, &map_w, &map_ws) || !encode(x, C::kBRows, BN, &map_x, &map_xs)) return context_free_fail(LM_ERR_CUDA, error.c_str());
+    const auto kernel = mx_matmul_kernel<BN, PAIR>;
+    static std::atomic<uint64_t> configured{0};  // devices whose limit is raised
+    if (const cudaError_t e = set_smem_limit_once(kernel, C::kSmemBytes, configured); e != cudaSuccess) return context_free_finish(e);
+    cudaLaunchConfig_t cfg{};
+    const int ctas = C::kCtas * a.split;
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles, kSms / ctas) * ctas));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = C::kSmemBytes;
+    cfg.stream = stream;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = static_cast<unsigned>(ctas);
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    cfg.attrs = &cluster;
+    cfg.numAttrs = ctas > 1 ? 1 : 0;
+    return context_free_finish(cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, map_ws, map_xs, a));
 }
 
 }  // namespace
@@ -404,13 +554,26 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
     if (out == nullptr || !aligned(out, elem_size(out_dtype)) || !aligned(offsets, 4) || x == nullptr || x_scales == nullptr || w == nullptr || w_scales == nullptr ||
         !aligned(x, 32) || !aligned(x_scales, 16) || !aligned(w, 32) || !aligned(w_scales, 16))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_mx_matmul: a null pointer, or data not 32-byte or scales not 16-byte aligned");
-    // The tile's width: groups are ragged, so half as much again as the average rows of a group keeps
-    // most of them in one tile (a second tile reads the group's weights again).
+    // The tile's width by the average rows of a group.  Groups are ragged, so a tile is wide enough for
+    // most of them: a second tile reads the group's weights again (64 experts of 2816 x 2048: at 12 rows a
+    // group 45 us with 16, 42 with 32, 46 with 64; at 24: 74, 48, 46; at 64: 85 with 32, 61 with 64,
+    // 60 with 128; from about 100 rows on pairs of CTAs read less: at 384 rows 174 against 195 us).
     const int64_t each = (rows + groups - 1) / groups;
-    const int bn = each <= 10 ? 16 : each <= 20 ? 32 : each <= 40 ? 64 : 128;
-    const int64_t m_blocks = (n + kBlockM - 1) / kBlockM;
-    const int64_t column_tiles = (rows + bn - 1) / bn + std::min<int64_t>(groups, rows) - 1;  // at most
-    if (column_tiles * m_blocks > INT32_MAX - kSms) return context_free_fail(LM_ERR_UNSUPPORTED, "lm_mx_matmul: more than 2^31 tiles");
+    int bn = each <= 6 ? 16 : each <= 18 ? 32 : each <= 56 ? 64 : 128;
+    const auto tiles = [&](int64_t m_blocks) { return m_blocks * ((rows + bn - 1) / bn + std::min<int64_t>(groups, rows) - 1); };  // at most
+    const int64_t m_blocks = (n + kBlockM - 1) / kBlockM, k_boxes = mx_padded_cols(k) / kBoxCols;
+    if (tiles(m_blocks) > INT32_MAX - kSms) return context_free_fail(LM_ERR_UNSUPPORTED, "lm_mx_matmul: more than 2^31 tiles");
+    const bool pair = each >= 112 && tiles(m_blocks) >= 8 * kSms;
+    // Fewer tiles than half the SMs: clusters of two or four CTAs share a tile's columns, at least four
+    // boxes each, and add their sums through distributed shared memory, without a workspace; after
+    // that, narrower tiles.  (One row, 10944 columns to 2048: one CTA a tile 20.6 us, two 14.4, four
+    // 10.7; eight, of which not all clusters fit the GPU at once, 15.6.  128 rows: four and 64 rows a tile
+    // 13.5 us, one and 16 rows 21.2.)
+    int split = 1;
+    for (;; bn /= 2) {
+        while (split < kMaxSplit && tiles(m_blocks) * split * 2 <= kSms && k_boxes >= 8 * split) split *= 2;
+        if (bn == 16 || tiles(m_blocks) * split * 2 > kSms) break;
+    }
     Args a{};
     a.offsets = offsets;
     a.out = out;
@@ -418,18 +581,20 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
     a.rows = static_cast<int>(rows);
     a.groups = groups;
     a.n = static_cast<int>(n);
-    a.k_boxes = static_cast<int>(mx_padded_cols(k) / kBoxCols);
+    a.k_boxes = static_cast<int>(k_boxes);
+    a.split = split;
     a.x_four_bit = x_format == LM_MX_E2M1;
     a.out_dtype = out_dtype;
+    a.out_pairs = out_stride % 2 == 0 && aligned(out, 4);
     if (const cudaError_t e = ops_status(&a.status); e != cudaSuccess) return context_free_finish(e);
     const Matrix mw{w, w_scales, true, groups * n}, mx{x, x_scales, x_format == LM_MX_E2M1, rows};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int64_t tiles = column_tiles * m_blocks;
+    if (pair) return launch<128, true>(mw, mx, k, a, tiles((n + 2 * kBlockM - 1) / (2 * kBlockM)), s);
     switch (bn) {
-        case 16: return launch<16>(mw, mx, k, a, tiles, s);
-        case 32: return launch<32>(mw, mx, k, a, tiles, s);
-        case 64: return launch<64>(mw, mx, k, a, tiles, s);
-        default: return launch<128>(mw, mx, k, a, tiles, s);
+        case 16: return launch<16, false>(mw, mx, k, a, tiles(m_blocks), s);
+        case 32: return launch<32, false>(mw, mx, k, a, tiles(m_blocks), s);
+        case 64: return launch<64, false>(mw, mx, k, a, tiles(m_blocks), s);
+        default: return launch<128, false>(mw, mx, k, a, tiles(m_blocks), s);
     }
 }
 

@@ -314,6 +314,16 @@ __device__ __forceinline__ void umma_mx(uint32_t d_tmem, uint64_t a_desc, uint64
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
         : "memory");
 }
+// The same over a CTA pair (M = 256, issued by the leader): each CTA holds half of A's rows with
+// their scales, half of B's rows, and the scales of all of B's rows.
+__device__ __forceinline__ void umma_mx_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa,
+                                             uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
 constexpr uint32_t kUmmaE4M3 = 0, kUmmaE2M1 = 5;  // operand formats
 __host__ __device__ constexpr uint32_t umma_idesc_mx(uint32_t a_format, uint32_t b_format, int M, int N, int scale_byte) {
     return (static_cast<uint32_t>(scale_byte) << 4)     // B's scale byte
@@ -351,6 +361,11 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar_addr) {
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t cluster_addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+    return v;
 }
 // TMA tile load into this CTA's shared memory whose completion is counted on an
 // mbarrier of the pair's leader CTA (`leader_bar` is a shared::cluster address).
@@ -391,6 +406,15 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t cluster_bar) {
                  : "memory");
 }
 
+// Arrives once on the mbarrier at this shared-memory offset in both CTAs of the pair when the
+// leader's MMAs issued so far complete.
+__device__ __forceinline__ void umma_commit_both(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
 // Named barrier for a subset of warps.
 __device__ __forceinline__ void named_bar_sync(uint32_t id, uint32_t threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");

@@ -180,6 +180,28 @@ def test_product_expert_layer_shapes():
         check_product(ops.mx_matmul(x, w, offsets, dtype=F32), x, w, cut, k, F32)
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("counts,n,k", [([4096], 4864, 300), ([700, 130, 0, 1, 1221, 128, 129, 1787], 4740, 1413), ([200] * 32, 3000, 1024), ([1000, 3100], 5001, 96)])
+def test_product_many_rows(counts, n, k, dtype, fmt):
+    """Enough rows a group and tiles for pairs of CTAs: ragged ends on every axis."""
+    x, w, offsets, cut = product_inputs(n + k, counts, n, k, fmt)
+    check_product(ops.mx_matmul(x, w, offsets, dtype=dtype), x, w, cut, k, dtype)
+
+
+@pytest.mark.parametrize("rows", [1, 5, 16, 17, 40, 64, 100, 128])
+@pytest.mark.parametrize("k", [1000, 1024, 2100, 4000, 10944])
+def test_product_long_columns(rows, k):
+    """Few tiles of many columns: clusters share a tile and add their sums, equal from call to call."""
+    for counts, n in (([rows], 200), ([rows, 0, 3], 130)):
+        x, w, offsets, cut = product_inputs(rows + k, counts, n, k, "e4m3")
+        out = ops.mx_matmul(x, w, offsets, dtype=F32)
+        check_product(out, x, w, cut, k, F32)
+        same_bits(ops.mx_matmul(x, w, offsets, dtype=F32), out)
+        for dtype in (BF16, F16):
+            check_product(ops.mx_matmul(x, w, offsets, dtype=dtype), x, w, cut, k, dtype)
+
+
 def test_product_leaves_other_rows_and_columns():
     """Rows of no group, and the columns between n and a wider output's stride, keep their values."""
     x, w, offsets, cut = product_inputs(1, [3, 0, 40], 70, 200, "e4m3", extra=9)
