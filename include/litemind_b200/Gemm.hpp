@@ -51,6 +51,14 @@ inline lm_status rms_norm(float* values, const float* weight, std::size_t count,
     return lm_gemm_rms_norm(values, weight, 1, static_cast<int64_t>(count), epsilon, stream);
 }
 
+/** sum = hidden + delta and its RMS norm to an MX matrix (see Mx.hpp), in one pass; out_bf16 may be null. */
+inline lm_status add_rms_norm_mx(const float* hidden, const float* delta, const float* weight, std::size_t rows,
+                                 std::size_t count, float epsilon, float* sum, std::uint16_t* out_bf16, int32_t format,
+                                 std::uint8_t* data, std::uint8_t* scales, void* stream = nullptr) {
+    return lm_gemm_add_rms_norm_mx(hidden, LM_DTYPE_F32, delta, LM_DTYPE_F32, weight, static_cast<int64_t>(rows),
+                                   static_cast<int64_t>(count), epsilon, sum, out_bf16, format, data, scales, stream);
+}
+
 /** In-place max-subtracted softmax. */
 inline lm_status softmax(float* values, std::size_t count, void* stream = nullptr) {
     return lm_gemm_softmax(values, 1, static_cast<int64_t>(count), stream);

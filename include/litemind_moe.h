@@ -380,7 +380,7 @@ lm_status lm_moe_route_static(const float* router, const uint16_t* x, int32_t to
  *             drops the pair (an expert held elsewhere, a padded token)
  *   offsets   int32 [experts + 1]: expert e's rows are offsets[e] .. offsets[e + 1] - 1
  *   at        int32 [tokens, top_k]: the pair's row, -1 when dropped
- * top_k <= LM_SORT_MAX_TOP_K, experts <= 1024, tokens x top_k < 2^31.
+ * top_k <= LM_SORT_MAX_TOP_K, experts <= 1024, tokens x top_k <= 2^31 - 1025.
  */
 #define LM_SORT_MAX_TOP_K 64
 lm_status lm_moe_sort_plan(const int32_t* topk_idx, int64_t tokens, int32_t top_k, int32_t experts, int32_t* offsets,
@@ -444,7 +444,7 @@ lm_status lm_mx_dequantize(const uint8_t* data, const uint8_t* scales, int32_t f
  *                (lm_moe_sort_plan's); NULL with groups = 1: all rows.  Values are clamped to
  *                [0, rows] and to ascending order; rows of no group are left as they were
  *   out          [rows, n], out_stride elements apart
- * k >= 1, groups <= LM_MX_MAX_GROUPS, groups * n < 2^31.  A NaN or infinity affects only its own row (x)
+ * rows <= 2^31 - 1025, k >= 1, groups <= LM_MX_MAX_GROUPS, groups * n <= 2^31 - 1025.  A NaN or infinity affects only its own row (x)
  * or its group's column (w).
  */
 lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_format, int64_t rows, const uint8_t* w,

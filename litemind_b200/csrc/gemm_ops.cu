@@ -193,11 +193,16 @@ unsigned blocks_for(int64_t n, int per) { return static_cast<unsigned>((n + per 
 }  // namespace
 
 const std::string& context_free_error() { return g_last_error; }
-lm_status context_free_fail(lm_status status, const char* message) {
-    g_last_error = message;
+lm_status context_free_fail(lm_status status, const char* message) noexcept {
+    try {
+        g_last_error = message;
+    } catch (...) {  // no memory for the text: the status still says what happened
+    }
     return status;
 }
-lm_status context_free_finish(cudaError_t e) { return finish(e); }
+lm_status context_free_finish(cudaError_t e) noexcept {
+    return e == cudaSuccess ? LM_OK : context_free_fail(LM_ERR_CUDA, cudaGetErrorString(e));
+}
 
 cudaError_t launch_rms_norm_rows(const float* in, float* out_f32, uint16_t* out_bf16, const float* weight, int rows,
                                  int count, float eps, cudaStream_t stream) {

@@ -281,8 +281,8 @@ cudaError_t launch_pack_swiglu(const uint16_t* gate, const uint16_t* up, const u
                                uint16_t* w13, uint16_t* w2, int sms, cudaStream_t stream);
 const std::string& context_free_error();
 // The same message for an entry point without a context: a refused argument, or a launch's status.
-lm_status context_free_fail(lm_status status, const char* message);
-lm_status context_free_finish(cudaError_t e);
+lm_status context_free_fail(lm_status status, const char* message) noexcept;
+lm_status context_free_finish(cudaError_t e) noexcept;
 // The current device's status word of the operators without a context (mx_matmul.cu), which
 // lm_ops_sync reads.
 cudaError_t ops_status(int** status);
@@ -306,9 +306,8 @@ cudaError_t set_smem_limit_once(Kernel kernel, int bytes, std::atomic<uint64_t>&
 // Host-side TMA descriptor encoding (tensor_map.cpp).
 bool encode_tensor_map_bf16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
                             uint32_t box_rows, uint32_t box_cols, std::string& error);
-bool encode_tensor_map_mx(CUtensorMap* map, const void* base, bool four_bit, uint64_t rows, uint64_t cols, uint32_t box_rows,
-                          std::string& error);
+bool encode_tensor_map_mx(CUtensorMap* map, const void* base, bool four_bit, uint64_t rows, uint64_t cols, uint32_t box_rows);
 bool encode_tensor_map_mx_scales(CUtensorMap* map, const void* base, uint64_t rows, uint64_t pitch, uint32_t box_rows,
-                                 uint32_t box_cols, std::string& error);
+                                 uint32_t box_cols);
 
 }  // namespace lm

@@ -8,7 +8,7 @@
 // group, pairs of CTAs walk tiles of 256 rows of W together, each bringing its half of both operands
 // (so that L2 delivers 47 bytes a cycle to an SM at the full rate of the MMA, not 92: it can 57).
 // A CTA's warps:
-//   0      TMA producer: a ring of stages of one or two boxes of 128 columns.  4-bit codes travel
+//   0      TMA producer: a ring of stages of two boxes of 128 columns.  4-bit codes travel
 //          packed (half a byte a column from HBM and L2); the TMA spreads them into the MMA's padded form.
 //   1      MMA issuer (of the pair's first CTA): four block-scaled MMAs of 32 columns a box
 //   2      scale producer: the scales of a chunk of boxes, to shared memory by TMA, ahead of the codes
@@ -502,13 +502,12 @@ template <int BN, bool PAIR>
 lm_status launch(const Matrix& w, const Matrix& x, int64_t k, const Args& a, int64_t tiles, cudaStream_t stream) {
     using C = Cfg<BN, PAIR>;
     CUtensorMap map_w, map_x, map_ws, map_xs;
-    std::string error;
     const uint64_t cols = static_cast<uint64_t>(mx_padded_cols(k)), pitch = static_cast<uint64_t>(mx_scale_pitch(k));
     const auto encode = [&](const Matrix& m, uint32_t box, uint32_t scale_box, CUtensorMap* codes, CUtensorMap* scales) {
-        return encode_tensor_map_mx(codes, m.codes, m.four_bit, static_cast<uint64_t>(m.rows), cols, box, error) &&
-               encode_tensor_map_mx_scales(scales, m.scales, static_cast<uint64_t>(m.rows), pitch, scale_box, C::kChunkBytes, error);
+        return encode_tensor_map_mx(codes, m.codes, m.four_bit, static_cast<uint64_t>(m.rows), cols, box) &&
+               encode_tensor_map_mx_scales(scales, m.scales, static_cast<uint64_t>(m.rows), pitch, scale_box, C::kChunkBytes);
     };
-    if (!encode(w, kBlockM, kBlockM, &map_w, &map_ws) || !encode(x, C::kBRows, BN, &map_x, &map_xs)) return context_free_fail(LM_ERR_CUDA, error.c_str());
+    if (!encode(w, kBlockM, kBlockM, &map_w, &map_ws) || !encode(x, C::kBRows, BN, &map_x, &map_xs)) return context_free_fail(LM_ERR_CUDA, "lm_mx_matmul: cuTensorMapEncodeTiled is unavailable or failed");
     const auto kernel = mx_matmul_kernel<BN, PAIR>;
     static std::atomic<uint64_t> configured{0};  // devices whose limit is raised
     if (const cudaError_t e = set_smem_limit_once(kernel, C::kSmemBytes, configured); e != cudaSuccess) return context_free_finish(e);

@@ -341,7 +341,7 @@ lm_status with_parts(int64_t tokens, int64_t parts, F&& f) {
 }
 
 bool sizes_ok(int64_t tokens, int32_t k) {
-    return tokens >= 0 && k > 0 && k <= LM_SORT_MAX_TOP_K && tokens <= INT32_MAX / k;
+    return tokens >= 0 && k > 0 && k <= LM_SORT_MAX_TOP_K && tokens <= (INT32_MAX - 1024) / k;  // 32-bit pair numbers, with room to step past the last
 }
 
 }  // namespace

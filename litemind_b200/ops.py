@@ -6,6 +6,7 @@ As in ``moe.py`` torch is the device-memory plumbing and all arithmetic runs in
 liblitemind_b200.so on the GPU.  Every call works on its tensors' device and that device's current
 stream, allocates its outputs with torch unless it is given them, and raises ``ValueError`` for an
 argument that does not fit (before any launch) or ``LiteMindError`` with the library's message.
+No autograd graph is recorded: the gradients are calls of their own.
 """
 from __future__ import annotations
 

@@ -6,6 +6,10 @@ Tolerances are derived, not fitted.  Quantisation and the sort are exact.  A sum
 is off by at most n 2^-23 of the sum of the terms' magnitudes (2^-23: an adder that truncates), and
 a result rounded to a type by half a step, finfo.eps / 2 of it.
 """
+import os
+import subprocess
+import sys
+
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -598,3 +602,110 @@ def test_two_streams_at_once():
     for i in range(2):
         for y in got[i]:
             same_bits(y, want[i])
+
+
+FIRST_CALLS = """
+import sys
+sys.path.insert(0, {root!r})
+import torch
+from litemind_b200 import ops
+
+torch.manual_seed(0)
+x, d, w = torch.randn(300, 512, device="cuda"), torch.randn(300, 512, device="cuda"), torch.ones(512, device="cuda")
+idx = torch.randint(0, 8, (1500, 2), device="cuda", dtype=torch.int32)
+wide = torch.randn(1500, 512, device="cuda")
+weights = torch.rand(1500, 2, device="cuda")
+torch.cuda.synchronize()
+
+def calls():
+    total, q, plain = ops.add_rms_norm(x, d, w, 1e-6, bf16=True)
+    m = ops.mx_quantize(x[:256], "e2m1")
+    y = ops.mx_matmul(q, m, dtype=torch.float32)
+    plan = ops.sort_plan(idx, 8)
+    rows = ops.sort_rows(wide, plan)
+    back = ops.unsort_rows(rows, plan, weights)
+    gr, gw = ops.unsort_rows_backward(back, rows, plan, weights)
+    return total, plain, ops.mx_dequantize(q), y, plan.offsets, plan.at, rows, back, gr, gw
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    captured = calls()
+graph.replay()
+torch.cuda.synchronize()
+for a, b in zip(captured, calls()):
+    assert torch.equal(a, b)
+ops.sync()
+print("equal")
+"""
+
+
+def test_first_calls_of_a_process_in_a_capture():
+    """Nothing has to be called once before a capture."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, "-c", FIRST_CALLS.format(root=root)], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and "equal" in res.stdout, res.stdout + res.stderr
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_product_output_alignment(dtype):
+    """Outputs that start on odd elements or have odd strides, every rest of a tile's columns."""
+    for n in (64, 95, 96, 127, 128, 129):
+        x, w, offsets, cut = product_inputs(n, [70, 0, 9], n, 160, "e4m3")
+        for width, start in ((n, 0), (n + 1, 0), (n + 1, 1), (n + 2, 1), (n + 4, 2)):
+            buffer = torch.full((79, width), 7.0, dtype=dtype, device="cuda")
+            check_product(ops.mx_matmul(x, w, offsets, dtype=dtype, out=buffer[:, start:start + n]), x, w, cut, 160, dtype)
+            assert (buffer[:, :start] == 7).all() and (buffer[:, start + n:] == 7).all()
+
+
+def test_rows_past_32_bits():
+    """Outputs and rows whose last elements lie past 2^31."""
+    rows, n, k = 70000, 40000, 64
+    x = ops.mx_quantize(normal(gen(1), rows, k, dtype=BF16), "e4m3")
+    w = ops.mx_quantize(normal(gen(2), 1, n, k, dtype=BF16), "e2m1")
+    out = ops.mx_matmul(x, w)
+    tail = ops.MxTensor(x.data[-300:].contiguous(), x.scales[-300:].contiguous(), k, "e4m3")
+    check_product(out[-300:], tail, w, [0, 300], k, BF16)
+    del out
+    n_rows, cols = 600000, 4096
+    big = torch.zeros(n_rows, cols, dtype=BF16, device="cuda")
+    at = torch.tensor([[n_rows - 1, 3], [n_rows - 2, -1], [n_rows - 5, 8]], dtype=torch.int32, device="cuda")
+    plan = ops.SortPlan(torch.zeros(2, dtype=torch.int32, device="cuda"), at)
+    v = normal(gen(3), 3, cols, dtype=BF16)
+    ops.sort_rows(v, plan, out=big)
+    for t, j, r in ((0, 0, n_rows - 1), (0, 1, 3), (1, 0, n_rows - 2), (2, 0, n_rows - 5), (2, 1, 8)):
+        assert torch.equal(big[r], v[t])
+    weights = torch.tensor([[1.0, 2.0], [4.0, 9.0], [0.5, 0.5]], device="cuda")
+    y = ops.unsort_rows(big, plan, weights, dtype=F32)
+    assert torch.equal(y, v.float() * torch.tensor([[3.0], [4.0], [1.0]], device="cuda"))
+    gr, gw = ops.unsort_rows_backward(v, big, plan, weights, out=big)
+    assert torch.equal(gr[n_rows - 2], v[1] * 4) and torch.equal(gr[8], v[2] * 0.5) and gw[1, 1] == 0
+
+
+def test_other_streams_and_plans_at_once():
+    """Plans of many pairs on two streams at once, and operators on a stream that is not the default."""
+    sets = [pairs(50 + i, 4000, 6, 160, 0.2) for i in range(2)]
+    want = [ref.sort_plan(s.cpu(), 160) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(ops.sort_plan(sets[i], 160))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for plan in got[i]:
+            assert torch.equal(plan.offsets.cpu(), want[i][0]) and torch.equal(plan.at.cpu(), want[i][1])
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_tensors_on_another_device():
+    with torch.cuda.device(0):
+        x = torch.randn(40, 256, device="cuda:1")
+        q = ops.mx_quantize(x, "e4m3")
+        w = ops.mx_quantize(torch.randn(64, 256, device="cuda:1"), "e2m1")
+        y = ops.mx_matmul(q, w, dtype=F32)
+        torch.cuda.synchronize(1)
+        check_product(y, q, ops.MxTensor(w.data[None], w.scales[None], 256, "e2m1"), [0, 40], 256, F32)
+        with pytest.raises(ValueError):
+            ops.mx_matmul(q, ops.mx_quantize(torch.randn(64, 256, device="cuda:0"), "e2m1"))

@@ -1,6 +1,6 @@
 """What the stand-alone operators refuse, through the C ABI without a GPU: every bad argument is
 answered with a status and a message before anything is launched, and empty inputs are no error."""
-import ctypes as C
+import subprocess
 
 import pytest
 
@@ -85,6 +85,14 @@ def test_sort(lib):
     refused(lib, "lm_moe_unsort_rows_backward", good, gy=[None, P + 1], rows=[None, P + 1], dtype=[0, 4], n=[-1], at=[None, P + 2], weights=[None, P + 1],
             tokens=[-1, 2**30], k=[0, 65], cols=[-1, 2**24 + 1], gr=[None, P + 1], gw=[None, P + 2])
     empty(lib, "lm_moe_unsort_rows_backward", good, tokens=[0])
+
+
+def test_cpp_forms(tmp_path):
+    """Mx.hpp and TokenSort.hpp compile as a user compiles them and answer as the C entries do."""
+    from tests.test_cpp_mirror import _compile
+
+    res = subprocess.run([_compile("MxTest", tmp_path)], capture_output=True, text=True, timeout=60)
+    assert res.returncode == 0, res.stdout + res.stderr
 
 
 def test_python_checks():
