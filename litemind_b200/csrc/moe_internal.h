@@ -306,8 +306,7 @@ cudaError_t set_smem_limit_once(Kernel kernel, int bytes, std::atomic<uint64_t>&
 // Host-side TMA descriptor encoding (tensor_map.cpp).
 bool encode_tensor_map_bf16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
                             uint32_t box_rows, uint32_t box_cols, std::string& error);
-bool encode_tensor_map_mx(CUtensorMap* map, const void* base, bool four_bit, uint64_t rows, uint64_t cols, uint32_t box_rows);
-bool encode_tensor_map_mx_scales(CUtensorMap* map, const void* base, uint64_t rows, uint64_t pitch, uint32_t box_rows,
-                                 uint32_t box_cols);
+bool encode_tensor_map_mx(CUtensorMap* map, const void* base, bool spread, uint64_t rows, uint64_t cols, uint32_t box_rows);
+bool encode_tensor_map_mx_scales(CUtensorMap* map, const void* base, uint64_t rows, uint64_t pitch, uint32_t box_rows);
 
 }  // namespace lm

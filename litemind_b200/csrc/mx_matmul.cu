@@ -28,24 +28,25 @@ namespace lm {
 namespace {
 
 constexpr int kBlockM = 128;
-constexpr int kBoxCols = 128;  // columns of a TMA box: one 128-byte row of the swizzled tiles
 constexpr int kThreads = 512;
 constexpr int kSms = 148;
 constexpr int kMaxSplit = 4;
-constexpr int kABoxBytes = kBlockM * kBoxCols;
+constexpr int kBoxRow = 128;  // bytes of a row of a TMA box in shared memory: one swizzled row
+constexpr int kABoxBytes = kBlockM * kBoxRow;
 
-template <int BN, bool PAIR>
+template <int BN, bool PAIR, bool FOUR>
 struct Cfg {
     static constexpr int kCtas = PAIR ? 2 : 1;
     static constexpr int kBRows = BN / kCtas;  // rows of X that a CTA brings
-    static constexpr int kBBoxBytes = kBRows * kBoxCols;
+    static constexpr int kBoxCols = FOUR ? 256 : 128;  // both operands packed, or 8 bits a column in shared memory
+    static constexpr int kBBoxBytes = kBRows * kBoxRow;
     static constexpr int kStageBoxes = 2;
     static constexpr int kStageBytes = kStageBoxes * (kABoxBytes + kBBoxBytes);
-    static constexpr int kBoxSf = 8;  // TMEM columns of a box's scales: 4 of W's, 4 of X's
-    // A chunk of scales: 4 bytes of a row for each box.  The TMEM that the two accumulators leave
-    // holds four chunks or more.
-    static constexpr int kChunkBoxes = 8, kChunkBytes = 4 * kChunkBoxes, kChunks = 3;
-    static constexpr int kSfCols = kChunkBoxes * kBoxSf, kSfGroups = 4;
+    // A chunk of scales: 1024 columns, 32 bytes a row, a word for each 128 columns (TMEM: 4 columns of
+    // W's words, 4 of X's).  What the two accumulators leave of TMEM holds four chunks or more.
+    static constexpr int kChunkBytes = 32, kChunkWords = kChunkBytes / 4, kBoxWords = kBoxCols / 128;
+    static constexpr int kChunkBoxes = kChunkWords / kBoxWords, kChunks = 3;
+    static constexpr int kSfCols = kChunkWords * 8, kSfGroups = 4;
     static constexpr int kScaleBytes = (kBlockM + BN) * kChunkBytes;
     static constexpr int kStagesFit = (216 * 1024 - kChunks * kScaleBytes) / kStageBytes;
     static constexpr int kStages = kStagesFit > 8 ? 8 : kStagesFit;
@@ -53,7 +54,7 @@ struct Cfg {
     static_assert(BN % 16 == 0 && BN >= 16 && 2 * BN + kSfGroups * kSfCols <= 512 && (!PAIR || BN % 32 == 0), "N of the MMA");
     static_assert(kBBoxBytes % 1024 == 0 || !PAIR, "swizzled tiles start on 1024 bytes");
     // Stages of one round of the issuer: two where a box's MMAs are short and the ring is long.
-    static constexpr int kRound = kStages >= 5 ? 2 : 1;
+    static constexpr int kRound = kStages >= 5 && !FOUR ? 2 : 1;
     static_assert(kStages >= 3 && kChunkBoxes % (kRound * kStageBoxes) == 0, "rings");
 };
 
@@ -64,7 +65,6 @@ struct Args {
     int rows, groups, n;
     int k_boxes;
     int split;  // CTAs (a cluster) that share a tile's boxes; more than 1: a cluster has one tile
-    int x_four_bit;
     int out_dtype;
     int out_pairs;  // 16-bit elements n, n + 1 (n even) lie on 4-byte boundaries
     int* status;
@@ -116,7 +116,7 @@ struct Tile {
     int n0;                 // first row of W_g for this CTA
 };
 
-template <int BN, bool PAIR>
+template <int BN, bool PAIR, bool FOUR>
 __device__ __forceinline__ Tile tile_at(const Args& a, const int* cut, const int* tiles, int t, int m_blocks, int rank) {
     const int ct = t / m_blocks;
     int lo = 0, hi = a.groups;  // tiles[lo] <= ct < tiles[hi]
@@ -128,7 +128,7 @@ __device__ __forceinline__ Tile tile_at(const Args& a, const int* cut, const int
     r.group = lo;
     r.row0 = cut[lo] + (ct - tiles[lo]) * BN;
     r.rows = min(BN, cut[lo + 1] - r.row0);
-    r.n0 = (t - ct * m_blocks) * kBlockM * Cfg<BN, PAIR>::kCtas + rank * kBlockM;
+    r.n0 = (t - ct * m_blocks) * kBlockM * Cfg<BN, PAIR, FOUR>::kCtas + rank * kBlockM;
     return r;
 }
 
@@ -166,11 +166,11 @@ __device__ __forceinline__ void store_columns(typename Elem<DT>::T* p, int64_t s
     }
 }
 
-template <int BN, bool PAIR>
+template <int BN, bool PAIR, bool FOUR>
 __global__ void __launch_bounds__(kThreads, 1)
     mx_matmul_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                      const __grid_constant__ CUtensorMap map_ws, const __grid_constant__ CUtensorMap map_xs, const Args a) {
-    using C = Cfg<BN, PAIR>;
+    using C = Cfg<BN, PAIR, FOUR>;
     constexpr int S = C::kStages, G = C::kSfGroups, B = C::kStageBoxes;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ int s_cut[LM_MX_MAX_GROUPS + 1], s_tiles[LM_MX_MAX_GROUPS + 1];
@@ -188,8 +188,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;
     const int split = PAIR ? 1 : a.split, part = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
     const int ctas = C::kCtas * split, first = blockIdx.x / ctas, step = gridDim.x / ctas;
-    // This CTA's boxes, from a multiple of four: 16 bytes of scales.
-    const int quads = (a.k_boxes + 3) / 4, box0 = quads * part / split * 4, boxes = min(a.k_boxes, quads * (part + 1) / split * 4) - box0;
+    // This CTA's boxes, from a multiple of 16 bytes of scales on.
+    constexpr int kUnit = 4 / C::kBoxWords;
+    const int units = (a.k_boxes + kUnit - 1) / kUnit, box0 = units * part / split * kUnit, boxes = min(a.k_boxes, units * (part + 1) / split * kUnit) - box0;
 
     const auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
         return mbar_wait(bar, parity, abort_flag, a.status, code);
@@ -199,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         else umma_commit(bar);
     };
     const auto arrive_first = [&](uint64_t* bar) {  // on the first CTA's barrier
-        if constexpr (PAIR) mbar_arrive_cluster(mapa_shared(smem_u32(bar), 0));
+        if constexpr (PAIR) mbar_arrive_cluster_tmem(mapa_shared(smem_u32(bar), 0));
         else mbar_arrive(bar);
     };
 
@@ -239,7 +240,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // In the issuing warps all lanes walk the loop and an elected one issues, so that descriptors and
     // addresses stay in uniform registers (under `if (lane == 0)` a stage took twice as long).
     if (warp == 0) {
-        const uint32_t box_bytes = kABoxBytes / 2 + (a.x_four_bit ? C::kBBoxBytes / 2 : C::kBBoxBytes);
+        const uint32_t box_bytes = (FOUR ? kABoxBytes : kABoxBytes / 2) + C::kBBoxBytes;  // spread codes count packed
+        constexpr int kColStep = FOUR ? kBoxRow : C::kBoxCols;  // a box in the map's elements: bytes when packed
         // Narrow tiles are for groups of few rows, whose weights are read once: they leave L2 first
         // (128 tokens over 64 experts: 43.8 -> 41.8 us; with 128 rows a tile it cost 7%).
         const uint64_t once = policy_evict_first();
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t phase = 0, issued = 0, issued_phase = 0;
         bool ok = true;
         for (int t = first; ok && t < total; t += step) {
-            const Tile tile = tile_at<BN, PAIR>(a, s_cut, s_tiles, t, m_blocks, rank);
+            const Tile tile = tile_at<BN, PAIR, FOUR>(a, s_cut, s_tiles, t, m_blocks, rank);
             const int w_row = tile.group * a.n + tile.n0;
             const int x_row = tile.row0 + rank * mma_n<PAIR>(tile.rows) / 2;
             for (int b = 0; b < boxes; b += B) {
@@ -260,12 +262,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         uint8_t *da = smem_a + (stage * B + i) * kABoxBytes, *db = smem_b + (stage * B + i) * C::kBBoxBytes;
                         if constexpr (PAIR) {
                             const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
-                            tma_load_2d_pair(da, &map_w, bar, (box0 + b + i) * kBoxCols, w_row);
-                            tma_load_2d_pair(db, &map_x, bar, (box0 + b + i) * kBoxCols, x_row);
+                            tma_load_2d_pair(da, &map_w, bar, (box0 + b + i) * kColStep, w_row);
+                            tma_load_2d_pair(db, &map_x, bar, (box0 + b + i) * kColStep, x_row);
                         } else {
-                            if constexpr (BN <= 64) tma_load_2d_hint(da, &map_w, &full[stage], (box0 + b + i) * kBoxCols, w_row, once);
-                            else tma_load_2d(da, &map_w, &full[stage], (box0 + b + i) * kBoxCols, w_row);
-                            tma_load_2d(db, &map_x, &full[stage], (box0 + b + i) * kBoxCols, x_row);
+                            if constexpr (BN <= 64) tma_load_2d_hint(da, &map_w, &full[stage], (box0 + b + i) * kColStep, w_row, once);
+                            else tma_load_2d(da, &map_w, &full[stage], (box0 + b + i) * kColStep, w_row);
+                            tma_load_2d(db, &map_x, &full[stage], (box0 + b + i) * kColStep, x_row);
                         }
                     }
                 }
@@ -282,14 +284,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         int stage = 0, sg = 0, acc = 0;
         uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
         bool ok = true, any = false, seen = false, sf_seen = false;
-        const uint32_t format = (a.x_four_bit ? kUmmaE2M1 : kUmmaE4M3) << 10;
         const uint64_t desc_a = umma_desc_sw128(smem_u32(smem_a)), desc_b = umma_desc_sw128(smem_u32(smem_b));
         constexpr int U = C::kRound;
         const auto after = [](int st, int by) { return st + by >= S ? st + by - S : st + by; };
         for (int t = first; ok && t < total; t += step) {
             int width = BN;  // a pair's MMAs are no wider than the tile's rows need; one CTA's take 50 cycles at least
-            if constexpr (PAIR) width = mma_n<PAIR>(tile_at<BN, PAIR>(a, s_cut, s_tiles, t, m_blocks, rank).rows);
-            const uint32_t shape = format | static_cast<uint32_t>(width >> 3) << 17;
+            if constexpr (PAIR) width = mma_n<PAIR>(tile_at<BN, PAIR, FOUR>(a, s_cut, s_tiles, t, m_blocks, rank).rows);
+            const uint32_t shape = static_cast<uint32_t>(width >> 3) << 17;
             ok = __all_sync(0xffffffffu, wait(&tmem_empty[acc], acc_phase ^ 1u, kDevTimeoutMma));
             const uint32_t d = tmem + acc * BN;
             for (int b = 0; ok && b < boxes; b += U * B) {
@@ -325,13 +326,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if (b + box < boxes) {
                                 const uint64_t da = desc_a + static_cast<uint32_t>((st * B + i) * (kABoxBytes >> 4));
                                 const uint64_t db = desc_b + static_cast<uint32_t>((st * B + i) * (C::kBBoxBytes >> 4));
-                                const uint32_t sf = tmem_sf + sg * C::kSfCols + (b % C::kChunkBoxes + box) * C::kBoxSf;
+                                const uint32_t sf = tmem_sf + sg * C::kSfCols + (b % C::kChunkBoxes + box) * C::kBoxWords * 8;
 #pragma unroll
-                                for (int kk = 0; kk < 4; ++kk) {  // 32 columns are 32 bytes, 2 in the descriptor's units
-                                    const uint32_t idesc = umma_idesc_mx(kUmmaE2M1, 0, kBlockM * C::kCtas, 0, kk) | shape;
-                                    const uint32_t add = b != 0 || box != 0 || kk != 0;
-                                    if constexpr (PAIR) umma_mx_pair(d, da + 2 * kk, db + 2 * kk, idesc, sf, sf + 4, add);
-                                    else umma_mx(d, da + 2 * kk, db + 2 * kk, idesc, sf, sf + 4, add);
+                                for (int kk = 0; kk < 4; ++kk) {  // 32 or 64 columns: 32 bytes, 2 in the descriptors' units
+                                    constexpr uint32_t kA = FOUR ? kUmmaPackedE2M1 : kUmmaE2M1, kB = FOUR ? kUmmaPackedE2M1 : kUmmaE4M3;
+                                    const uint32_t idesc = umma_idesc_mx(kA, kB, kBlockM * C::kCtas, 0, FOUR ? kk % 2 * 2 : kk) | shape;
+                                    const uint32_t word = sf + (FOUR ? kk / 2 * 8 : 0);
+                                    umma_mx<PAIR, FOUR>(d, da + 2 * kk, db + 2 * kk, idesc, word, word + 4, b != 0 || box != 0 || kk != 0);
                                 }
                             }
                         }
@@ -358,15 +359,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t phase = 0, issued = 0, issued_phase = 0;
         bool ok = true;
         for (int t = first; ok && t < total; t += step) {
-            const Tile tile = tile_at<BN, PAIR>(a, s_cut, s_tiles, t, m_blocks, rank);
+            const Tile tile = tile_at<BN, PAIR, FOUR>(a, s_cut, s_tiles, t, m_blocks, rank);
             for (int b = 0; b < boxes; b += C::kChunkBoxes) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&chunk_empty[chunk], phase ^ 1u, abort_flag, a.status, kDevTimeoutProducer));
                 if (!ok) break;
                 if (elect_one()) {
                     uint8_t* dst = smem_s + chunk * C::kScaleBytes;
                     mbar_arrive_expect_tx(&chunk_full[chunk], C::kScaleBytes);
-                    tma_load_2d(dst, &map_ws, &chunk_full[chunk], (box0 + b) * 4, tile.group * a.n + tile.n0);
-                    tma_load_2d(dst + kBlockM * C::kChunkBytes, &map_xs, &chunk_full[chunk], (box0 + b) * 4, tile.row0);
+                    tma_load_2d(dst, &map_ws, &chunk_full[chunk], (box0 + b) * C::kBoxWords * 4, tile.group * a.n + tile.n0);
+                    tma_load_2d(dst + kBlockM * C::kChunkBytes, &map_xs, &chunk_full[chunk], (box0 + b) * C::kBoxWords * 4, tile.row0);
                 }
                 __syncwarp();
                 issued |= 1u << chunk;
@@ -390,18 +391,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 ok = __all_sync(0xffffffffu, ok && wait(&sf_empty[sg], phase ^ 1u, kDevTimeoutProducer));
                 if (!ok) break;
                 tc_fence_after();
+                // 16 bytes of a row, its scales of 512 columns, at a time; the TMA's 32-byte swizzle swaps
+                // the halves of every second four rows, so that eight lanes reach all banks (with plain
+                // rows a chunk took 900 to 2000 cycles, the longest step of most products).
                 const uint8_t* src = smem_s + chunk * C::kScaleBytes + lane * C::kChunkBytes;
 #pragma unroll
-                for (int h = 0; h < C::kChunkBoxes / 2; ++h) {  // 8 bytes of a row are its scales in two boxes
-                    uint32_t r[16];
+                for (int h = 0; h < 2; ++h) {
+                    const uint8_t* at = src + 16 * (h ^ (lane >> 2 & 1));
+                    uint4 w[4], x[4];
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(src + 32 * c * C::kChunkBytes + 8 * h);
-                        uint2 x = make_uint2(0u, 0u);
-                        if (c < kXRows && (BN >= 32 || lane < BN)) x = *reinterpret_cast<const uint2*>(src + (kBlockM + 32 * c) * C::kChunkBytes + 8 * h);
-                        r[c] = w.x, r[8 + c] = w.y, r[4 + c] = x.x, r[12 + c] = x.y;
+                        w[c] = *reinterpret_cast<const uint4*>(at + 32 * c * C::kChunkBytes);
+                        x[c] = make_uint4(0u, 0u, 0u, 0u);
+                        if (c < kXRows && (BN >= 32 || lane < BN)) x[c] = *reinterpret_cast<const uint4*>(at + (kBlockM + 32 * c) * C::kChunkBytes);
                     }
-                    tmem_st16(tmem_sf + quad + sg * C::kSfCols + 16 * h, r);
+                    uint32_t r[16];
+                    const uint32_t to = tmem_sf + quad + sg * C::kSfCols + 32 * h;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) r[c] = w[c].x, r[4 + c] = x[c].x, r[8 + c] = w[c].y, r[12 + c] = x[c].y;
+                    tmem_st16(to, r);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) r[c] = w[c].z, r[4 + c] = x[c].z, r[8 + c] = w[c].w, r[12 + c] = x[c].w;
+                    tmem_st16(to + 16, r);
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -420,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int acc = 0;
         uint32_t acc_phase = 0;
         for (int t = first; t < total; t += step) {
-            const Tile tile = tile_at<BN, PAIR>(a, s_cut, s_tiles, t, m_blocks, rank);
+            const Tile tile = tile_at<BN, PAIR, FOUR>(a, s_cut, s_tiles, t, m_blocks, rank);
             int go = 1;
             if (lane == 0) go = wait(&tmem_full[acc], acc_phase, kDevTimeoutEpilogue);
             if (__shfl_sync(0xffffffffu, go, 0) == 0) break;
@@ -459,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncthreads();
             cluster_sync();
             if (first < total) {
-                const Tile tile = tile_at<BN, PAIR>(a, s_cut, s_tiles, first, m_blocks, rank);
+                const Tile tile = tile_at<BN, PAIR, FOUR>(a, s_cut, s_tiles, first, m_blocks, rank);
                 for (int i = part * kThreads + threadIdx.x; i < tile.rows * kBlockM; i += split * kThreads) {
                     float sum = 0.0f, v[kMaxSplit];
 #pragma unroll
@@ -494,21 +505,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 struct Matrix {
     const uint8_t* codes;
     const uint8_t* scales;
-    bool four_bit;
     int64_t rows;
 };
 
-template <int BN, bool PAIR>
+template <int BN, bool PAIR, bool FOUR>
 lm_status launch(const Matrix& w, const Matrix& x, int64_t k, const Args& a, int64_t tiles, cudaStream_t stream) {
-    using C = Cfg<BN, PAIR>;
+    using C = Cfg<BN, PAIR, FOUR>;
     CUtensorMap map_w, map_x, map_ws, map_xs;
     const uint64_t cols = static_cast<uint64_t>(mx_padded_cols(k)), pitch = static_cast<uint64_t>(mx_scale_pitch(k));
     const auto encode = [&](const Matrix& m, uint32_t box, uint32_t scale_box, CUtensorMap* codes, CUtensorMap* scales) {
-        return encode_tensor_map_mx(codes, m.codes, m.four_bit, static_cast<uint64_t>(m.rows), cols, box) &&
-               encode_tensor_map_mx_scales(scales, m.scales, static_cast<uint64_t>(m.rows), pitch, scale_box, C::kChunkBytes);
+        const bool spread = !FOUR && codes == &map_w;
+        return encode_tensor_map_mx(codes, m.codes, spread, static_cast<uint64_t>(m.rows), FOUR ? cols / 2 : cols, box) &&
+               encode_tensor_map_mx_scales(scales, m.scales, static_cast<uint64_t>(m.rows), pitch, scale_box);
     };
     if (!encode(w, kBlockM, kBlockM, &map_w, &map_ws) || !encode(x, C::kBRows, BN, &map_x, &map_xs)) return context_free_fail(LM_ERR_CUDA, "lm_mx_matmul: cuTensorMapEncodeTiled is unavailable or failed");
-    const auto kernel = mx_matmul_kernel<BN, PAIR>;
+    const auto kernel = mx_matmul_kernel<BN, PAIR, FOUR>;
     static std::atomic<uint64_t> configured{0};  // devices whose limit is raised
     if (const cudaError_t e = set_smem_limit_once(kernel, C::kSmemBytes, configured); e != cudaSuccess) return context_free_finish(e);
     cudaLaunchConfig_t cfg{};
@@ -560,19 +571,20 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
     const int64_t each = (rows + groups - 1) / groups;
     int bn = each <= 6 ? 16 : each <= 18 ? 32 : each <= 56 ? 64 : 128;
     const auto tiles = [&](int64_t m_blocks) { return m_blocks * ((rows + bn - 1) / bn + std::min<int64_t>(groups, rows) - 1); };  // at most
-    const int64_t m_blocks = (n + kBlockM - 1) / kBlockM, k_boxes = mx_padded_cols(k) / kBoxCols;
+    const int64_t m_blocks = (n + kBlockM - 1) / kBlockM, k_words = mx_padded_cols(k) / 128;  // of scales
     if (tiles(m_blocks) > INT32_MAX - kSms) return context_free_fail(LM_ERR_UNSUPPORTED, "lm_mx_matmul: more than 2^31 tiles");
     const bool pair = each >= 112 && tiles(m_blocks) >= 8 * kSms;
-    // Fewer tiles than half the SMs: clusters of two or four CTAs share a tile's columns, at least four
-    // boxes each, and add their sums through distributed shared memory, without a workspace; after
+    // Fewer tiles than half the SMs: clusters of two or four CTAs share a tile's columns, at least 512
+    // each, and add their sums through distributed shared memory, without a workspace; after
     // that, narrower tiles.  (One row, 10944 columns to 2048: one CTA a tile 20.6 us, two 14.4, four
     // 10.7; eight, of which not all clusters fit the GPU at once, 15.6.  128 rows: four and 64 rows a tile
     // 13.5 us, one and 16 rows 21.2.)
     int split = 1;
     for (;; bn /= 2) {
-        while (split < kMaxSplit && tiles(m_blocks) * split * 2 <= kSms && k_boxes >= 8 * split) split *= 2;
+        while (split < kMaxSplit && tiles(m_blocks) * split * 2 <= kSms && k_words >= 8 * split) split *= 2;
         if (bn == 16 || tiles(m_blocks) * split * 2 > kSms) break;
     }
+    const bool four = x_format == LM_MX_E2M1;
     Args a{};
     a.offsets = offsets;
     a.out = out;
@@ -580,21 +592,23 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
     a.rows = static_cast<int>(rows);
     a.groups = groups;
     a.n = static_cast<int>(n);
-    a.k_boxes = static_cast<int>(k_boxes);
+    a.k_boxes = static_cast<int>(four ? (k_words + 1) / 2 : k_words);
     a.split = split;
-    a.x_four_bit = x_format == LM_MX_E2M1;
     a.out_dtype = out_dtype;
     a.out_pairs = out_stride % 2 == 0 && aligned(out, 4);
     if (const cudaError_t e = ops_status(&a.status); e != cudaSuccess) return context_free_finish(e);
-    const Matrix mw{w, w_scales, true, groups * n}, mx{x, x_scales, x_format == LM_MX_E2M1, rows};
+    const Matrix mw{w, w_scales, groups * n}, mx{x, x_scales, rows};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (pair) return launch<128, true>(mw, mx, k, a, tiles((n + 2 * kBlockM - 1) / (2 * kBlockM)), s);
-    switch (bn) {
-        case 16: return launch<16, false>(mw, mx, k, a, tiles(m_blocks), s);
-        case 32: return launch<32, false>(mw, mx, k, a, tiles(m_blocks), s);
-        case 64: return launch<64, false>(mw, mx, k, a, tiles(m_blocks), s);
-        default: return launch<128, false>(mw, mx, k, a, tiles(m_blocks), s);
-    }
+    lm_status st = LM_OK;
+    with_bool(four, [&](auto f) {
+        constexpr bool FOUR = decltype(f)::value;
+        if (pair) st = launch<128, true, FOUR>(mw, mx, k, a, tiles((n + 2 * kBlockM - 1) / (2 * kBlockM)), s);
+        else if (bn == 16) st = launch<16, false, FOUR>(mw, mx, k, a, tiles(m_blocks), s);
+        else if (bn == 32) st = launch<32, false, FOUR>(mw, mx, k, a, tiles(m_blocks), s);
+        else if (bn == 64) st = launch<64, false, FOUR>(mw, mx, k, a, tiles(m_blocks), s);
+        else st = launch<128, false, FOUR>(mw, mx, k, a, tiles(m_blocks), s);
+    });
+    return st;
 }
 
 lm_status lm_ops_sync(void* stream) {

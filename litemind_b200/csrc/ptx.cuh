@@ -301,30 +301,30 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // ── block-scaled MMA: 8- and 4-bit operands with E8M0 scales of 32 columns ──
-// D[tmem] (+)= (A * 2^sa) * (B * 2^sb)^T over 32 columns (kind::mxf8f6f4).  A 4-bit operand sits in
-// shared memory as TMA's 16U4_ALIGN16B type writes it: 16 codes in 8 bytes, then 8 unused bytes, so
-// that 128 columns fill the same 128-byte swizzled row as 8-bit codes do.  Scales sit in TMEM: word
-// (lane i, column c) of `sfa` holds four scale bytes of row 32 c + i, the same in each 32-lane
-// quadrant; the descriptor names the byte.
+// D[tmem] (+)= (A * 2^sa) * (B * 2^sb)^T, with A and B in shared memory as 128-byte swizzled rows.
+//   FOUR = false  kind::mxf8f6f4, 32 columns: 8-bit codes, or 4-bit ones spread as TMA's 16U4_ALIGN16B
+//                 type writes them (16 codes in 8 bytes, then 8 unused bytes)
+//   FOUR = true   kind::mxf4, 64 columns: both operands 4-bit and packed
+// Scales sit in TMEM: word (lane i, column c) of `sfa` holds four scale bytes of row 32 c + i, the same
+// in each 32-lane quadrant; the descriptor names the byte, or the first of the two bytes of 64 columns.
+// PAIR: over a CTA pair (M = 256, issued by the first): each CTA holds half of A's rows with their
+// scales, half of B's rows, and the scales of all of B's rows.
+template <bool PAIR, bool FOUR>
 __device__ __forceinline__ void umma_mx(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa,
                                         uint32_t sfb, uint32_t accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
+#define LM_UMMA_MX(CTAS, KIND)                                                                                             \
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"                                                            \
+                 " tcgen05.mma.cta_group::" CTAS ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d_tmem),     \
+                 "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                                  \
+                 : "memory")
+    if constexpr (FOUR && PAIR) LM_UMMA_MX("2", "mxf4.block_scale.scale_vec::2X");
+    else if constexpr (FOUR) LM_UMMA_MX("1", "mxf4.block_scale.scale_vec::2X");
+    else if constexpr (PAIR) LM_UMMA_MX("2", "mxf8f6f4.block_scale.scale_vec::1X");
+    else LM_UMMA_MX("1", "mxf8f6f4.block_scale.scale_vec::1X");
+#undef LM_UMMA_MX
 }
-// The same over a CTA pair (M = 256, issued by the leader): each CTA holds half of A's rows with
-// their scales, half of B's rows, and the scales of all of B's rows.
-__device__ __forceinline__ void umma_mx_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa,
-                                             uint32_t sfb, uint32_t accumulate) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
-}
-constexpr uint32_t kUmmaE4M3 = 0, kUmmaE2M1 = 5;  // operand formats
+// Operand formats of kind::mxf8f6f4 and of kind::mxf4.
+constexpr uint32_t kUmmaE4M3 = 0, kUmmaE2M1 = 5, kUmmaPackedE2M1 = 1;
 __host__ __device__ constexpr uint32_t umma_idesc_mx(uint32_t a_format, uint32_t b_format, int M, int N, int scale_byte) {
     return (static_cast<uint32_t>(scale_byte) << 4)     // B's scale byte
            | (a_format << 7) | (b_format << 10)
@@ -358,6 +358,11 @@ __device__ __forceinline__ uint32_t mapa_shared(uint32_t smem_addr, uint32_t ran
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar_addr) : "memory");
+}
+// The same with this CTA's scope: for a barrier that orders TMEM accesses only (between the tcgen05
+// fences).  The release at cluster scope waits for the thread's earlier memory accesses, 1700 cycles.
+__device__ __forceinline__ void mbar_arrive_cluster_tmem(uint32_t cluster_bar_addr) {
+    asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar_addr) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");

@@ -61,32 +61,32 @@ bool encode_tensor_map_bf16(CUtensorMap* map, const void* base, uint64_t rows, u
     return true;
 }
 
-// An MX matrix's codes, [rows, cols] with cols a multiple of 128, read in boxes of 128 columns.
-// 4-bit codes arrive as the block-scaled MMA reads them (8 bytes of codes, 8 of gap); a box then
-// completes its packed bytes, rows x 64, on the barrier.
-bool encode_tensor_map_mx(CUtensorMap* map, const void* base, bool four_bit, uint64_t rows, uint64_t cols, uint32_t box_rows) {
+// An MX matrix's codes, read in boxes of 128 elements a row.  spread: [rows, cols] 4-bit codes, cols a
+// multiple of 128, that arrive as kind::mxf8f6f4 reads them (8 bytes of codes, 8 of gap); a box then
+// completes its packed bytes, rows x 64, on the barrier.  Else [rows, cols] bytes.
+bool encode_tensor_map_mx(CUtensorMap* map, const void* base, bool spread, uint64_t rows, uint64_t cols, uint32_t box_rows) {
     auto fn = encode_fn();
     if (fn == nullptr) return false;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
-    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(four_bit ? cols / 2 : cols)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(spread ? cols / 2 : cols)};
     const cuuint32_t box[2] = {128, box_rows};
     const cuuint32_t elem_strides[2] = {1, 1};
-    return fn(map, four_bit ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
+    return fn(map, spread ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims,
               strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// An MX matrix's scales, [rows, pitch] bytes, read in boxes of box_cols bytes without a swizzle.
-bool encode_tensor_map_mx_scales(CUtensorMap* map, const void* base, uint64_t rows, uint64_t pitch, uint32_t box_rows,
-                                 uint32_t box_cols) {
+// An MX matrix's scales, [rows, pitch] bytes, read in boxes of 32 bytes a row with the 32-byte swizzle:
+// the 16-byte halves of rows 4 to 7 of every eight change places.
+bool encode_tensor_map_mx_scales(CUtensorMap* map, const void* base, uint64_t rows, uint64_t pitch, uint32_t box_rows) {
     auto fn = encode_fn();
     if (fn == nullptr) return false;
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(pitch), static_cast<cuuint64_t>(rows)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
-    const cuuint32_t box[2] = {box_cols, box_rows};
+    const cuuint32_t box[2] = {32, box_rows};
     const cuuint32_t elem_strides[2] = {1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem_strides,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
