@@ -523,7 +523,7 @@ lm_status launch(const Matrix& w, const Matrix& x, int64_t k, const Args& a, int
     static std::atomic<uint64_t> configured{0};  // devices whose limit is raised
     if (const cudaError_t e = set_smem_limit_once(kernel, C::kSmemBytes, configured); e != cudaSuccess) return context_free_finish(e);
     cudaLaunchConfig_t cfg{};
-    const int ctas = C::kCtas * a.split;
+    const int ctas = PAIR ? 2 : a.split;
     cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>(tiles, kSms / ctas) * ctas));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = C::kSmemBytes;
@@ -565,24 +565,27 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
         !aligned(x, 32) || !aligned(x_scales, 16) || !aligned(w, 32) || !aligned(w_scales, 16))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_mx_matmul: a null pointer, or data not 32-byte or scales not 16-byte aligned");
     // The tile's width by the average rows of a group.  Groups are ragged, so a tile is wide enough for
-    // most of them: a second tile reads the group's weights again (64 experts of 2816 x 2048: at 12 rows a
-    // group 45 us with 16, 42 with 32, 46 with 64; at 24: 74, 48, 46; at 64: 85 with 32, 61 with 64,
-    // 60 with 128; from about 100 rows on pairs of CTAs read less: at 384 rows 174 against 195 us).
+    // most of them: a second tile reads the group's weights again.  (64 experts of 2816 x 2048, us with
+    // 16, 32, 64 rows a tile and with a pair's 128: 4 rows a group 39, 40, 45, 49; 16: 51, 40, 44, 47;
+    // 40: 107, 69, 49, 50; 64: 140, 84, 61, 50.)
     const int64_t each = (rows + groups - 1) / groups;
-    int bn = each <= 6 ? 16 : each <= 18 ? 32 : each <= 56 ? 64 : 128;
+    int bn = each <= 6 ? 16 : each <= 18 ? 32 : each <= 40 ? 64 : 128;
     const auto tiles = [&](int64_t m_blocks) { return m_blocks * ((rows + bn - 1) / bn + std::min<int64_t>(groups, rows) - 1); };  // at most
     const int64_t m_blocks = (n + kBlockM - 1) / kBlockM, k_words = mx_padded_cols(k) / 128;  // of scales
     if (tiles(m_blocks) > INT32_MAX - kSms) return context_free_fail(LM_ERR_UNSUPPORTED, "lm_mx_matmul: more than 2^31 tiles");
-    const bool pair = each >= 112 && tiles(m_blocks) >= 8 * kSms;
-    // Fewer tiles than half the SMs: clusters of two or four CTAs share a tile's columns, at least 512
-    // each, and add their sums through distributed shared memory, without a workspace; after
-    // that, narrower tiles.  (One row, 10944 columns to 2048: one CTA a tile 20.6 us, two 14.4, four
-    // 10.7; eight, of which not all clusters fit the GPU at once, 15.6.  128 rows: four and 64 rows a tile
-    // 13.5 us, one and 16 rows 21.2.)
+    // Pairs of CTAs where 128 rows a tile give them work (384 rows a group: 196 us without, 163 with).
+    const bool pair = bn == 128 && tiles(m_blocks) * 2 > kSms;
+    // Fewer tiles than half the SMs: narrower tiles, and clusters of two or four CTAs that share a tile's
+    // columns, at least 512 each, and add their sums through distributed shared memory, without a
+    // workspace.  Many columns are shared before tiles get narrower, few after.  (One row, 10944 columns
+    // to 2048: one CTA a tile 20.6 us, two 14.4, four 10.7; eight, of which not all clusters fit the GPU at
+    // once, 15.6.  128 rows of them: 64 rows a tile shared by four 13.5 us, 16 rows unshared 21.2.  256 rows
+    // of 2048 columns: 128 shared by four 10.6, 32 unshared 8.4.)
     int split = 1;
-    for (;; bn /= 2) {
-        while (split < kMaxSplit && tiles(m_blocks) * split * 2 <= kSms && k_words >= 8 * split) split *= 2;
-        if (bn == 16 || tiles(m_blocks) * split * 2 > kSms) break;
+    for (const bool share_first = k_words >= 32; !pair; bn /= 2) {
+        const auto few = [&] { return tiles(m_blocks) * split * 2 <= kSms; };
+        while ((share_first || bn == 16) && split < kMaxSplit && few() && k_words >= 8 * split) split *= 2;
+        if (bn == 16 || !few()) break;
     }
     const bool four = x_format == LM_MX_E2M1;
     Args a{};
