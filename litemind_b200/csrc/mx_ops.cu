@@ -328,11 +328,20 @@ lm_status lm_gemm_add_rms_norm_mx(const void* hidden, int32_t dtype, const void*
                     static_cast<const T*>(hidden), delta, delta_dtype == LM_DTYPE_F32, weight, count, 1.0 / static_cast<double>(count), epsilon, static_cast<T*>(sum),
                     reinterpret_cast<__nv_bfloat16*>(out_bf16), format, data, mx_data_pitch(format, count), scales, mx_scale_pitch(count));
             };
-            const auto one = std::integral_constant<int, 1>{};
-            if (wide <= 2048) go(std::integral_constant<int, 256>{}, one);
-            else if (wide <= 4096) go(std::integral_constant<int, 512>{}, one);
-            else if (wide <= 8192) go(std::integral_constant<int, 1024>{}, one);
-            else go(std::integral_constant<int, 1024>{}, std::integral_constant<int, 0>{});
+            // Few idle threads, then several CTAs an SM: bf16 rows of 1024 took 31 us with 128 threads and
+            // 49 with 256 (20000 rows), of 6144 52 with 384 and 65 with 1024 (4096 rows), and f32 rows of
+            // 8192 138 with 512 and 157 with 1024 (8192 rows).  Two stretches a thread lost where one of
+            // 512 threads covers the row (60 us, 57 at 8192 x 4096).
+            using std::integral_constant;
+            const integral_constant<int, 1> one;
+            const integral_constant<int, 2> two;
+            if (wide <= 1024) go(integral_constant<int, 128>{}, one);
+            else if (wide <= 2048) go(integral_constant<int, 256>{}, one);
+            else if (wide <= 4096) go(integral_constant<int, 512>{}, one);
+            else if (wide <= 6144) go(integral_constant<int, 384>{}, two);
+            else if (wide <= 8192) go(integral_constant<int, 512>{}, two);
+            else if (wide <= 16384) go(integral_constant<int, 1024>{}, two);
+            else go(integral_constant<int, 512>{}, integral_constant<int, 0>{});
         });
     });
     return context_free_finish(cudaGetLastError());
