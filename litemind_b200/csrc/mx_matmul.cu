@@ -5,18 +5,21 @@
 //
 // The weights are the MMA's M side, so that a few rows of X cost a narrow N instead of a padded M.
 // One persistent CTA an SM walks the tiles (group, BN rows of X, 128 rows of W); for many rows a
-// group, pairs of CTAs walk tiles of 256 rows of W together, each bringing its half of both operands
-// (so that L2 delivers 47 bytes a cycle to an SM at the full rate of the MMA, not 92: it can 57).
+// group, pairs of CTAs walk tiles of 256 rows of W by 128 of X together, each bringing its half of
+// both operands (L2 delivers about 57 bytes a cycle to an SM; at the full rate of the MMA a CTA of
+// its own asks for 92 and one of a pair for 62).
+// E4M3 rows of X take kind::mxf8f6f4, whose 4-bit operand is padded to a byte a code: W's codes
+// travel packed and the TMA spreads them in shared memory.  E2M1 rows take kind::mxf4 with both
+// operands packed, half the shared memory and half the MMAs (dense 4096 x 10944 x 2048: 51 us, 84
+// with E4M3 rows).
 // A CTA's warps:
-//   0      TMA producer: a ring of stages of two boxes of 128 columns.  4-bit codes travel
-//          packed (half a byte a column from HBM and L2); the TMA spreads them into the MMA's padded form.
-//   1      MMA issuer (of the pair's first CTA): four block-scaled MMAs of 32 columns a box
+//   0      TMA producer: a ring of stages of two boxes of 128 bytes a row
+//   1      MMA issuer (of the pair's first CTA): four block-scaled MMAs a box
 //   2      scale producer: the scales of a chunk of boxes, to shared memory by TMA, ahead of the codes
 //   4-7    scales from shared memory to TMEM, each warp to its own quadrant
 //   8-15   epilogue: TMEM to registers to out, rounded once; two warps a quadrant share the rows of X
 // A stage costs the issuer about 400 cycles of waits, descriptors and commits whatever its width,
-// and the four MMAs of a box take 200 (N = 16) to 256 (N = 128) or, in a pair, 512 (N = 256): hence
-// two boxes a stage where they are short.
+// and the four MMAs of a box take 200 (N = 16) to 256 (N = 128): hence two boxes a stage.
 // Every wait is bounded (ptx.cuh): a pipeline that stalls records a status for lm_ops_sync.
 #include "moe_internal.h"
 #include "mx_block.cuh"
@@ -566,28 +569,29 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_mx_matmul: a null pointer, or data not 32-byte or scales not 16-byte aligned");
     // The tile's width by the average rows of a group.  Groups are ragged, so a tile is wide enough for
     // most of them: a second tile reads the group's weights again.  (64 experts of 2816 x 2048, us with
-    // 16, 32, 64 rows a tile and with a pair's 128: 4 rows a group 39, 40, 45, 49; 16: 51, 40, 44, 47;
-    // 40: 107, 69, 49, 50; 64: 140, 84, 61, 50.)
+    // 16, 32, 64 rows a tile and with a pair's 128, E4M3 rows: 4 a group 39, 41, 45, 49; 16: 51, 40, 44,
+    // 47; 40: 101, 64, 45, 49; 48: 64 rows 48, a pair 49; 59: 55 and 50.  Packed E2M1 rows: 4 a group 33,
+    // 34, 32, 41; 16: 35, 34, 33, 40; 59: 64 rows 36, a pair 41; 66: 42 and 42.)
+    const bool four = x_format == LM_MX_E2M1;
     const int64_t each = (rows + groups - 1) / groups;
-    int bn = each <= 6 ? 16 : each <= 18 ? 32 : each <= 40 ? 64 : 128;
+    int bn = each <= 6 ? 16 : each <= 18 ? 32 : each <= (four ? 64 : 48) ? 64 : 128;
     const auto tiles = [&](int64_t m_blocks) { return m_blocks * ((rows + bn - 1) / bn + std::min<int64_t>(groups, rows) - 1); };  // at most
     const int64_t m_blocks = (n + kBlockM - 1) / kBlockM, k_words = mx_padded_cols(k) / 128;  // of scales
     if (tiles(m_blocks) > INT32_MAX - kSms) return context_free_fail(LM_ERR_UNSUPPORTED, "lm_mx_matmul: more than 2^31 tiles");
-    // Pairs of CTAs where 128 rows a tile give them work (384 rows a group: 196 us without, 163 with).
+    // Pairs of CTAs where 128 rows a tile give them work (384 rows a group: 195 us without, 170 with).
     const bool pair = bn == 128 && tiles(m_blocks) * 2 > kSms;
     // Fewer tiles than half the SMs: narrower tiles, and clusters of two or four CTAs that share a tile's
     // columns, at least 512 each, and add their sums through distributed shared memory, without a
     // workspace.  Many columns are shared before tiles get narrower, few after.  (One row, 10944 columns
-    // to 2048: one CTA a tile 20.6 us, two 14.4, four 10.7; eight, of which not all clusters fit the GPU at
-    // once, 15.6.  128 rows of them: 64 rows a tile shared by four 13.5 us, 16 rows unshared 21.2.  256 rows
-    // of 2048 columns: 128 shared by four 10.6, 32 unshared 8.4.)
+    // to 2048: one CTA a tile 24 us, two 17, four 12.6; eight, of which not all clusters fit the GPU at
+    // once, were slower than four.  128 rows of them: 64 rows a tile shared by four 14 us, 16 rows unshared
+    // 23.  256 rows of 2048 columns: 128 shared by four 10.6, 32 unshared 8.8.)
     int split = 1;
     for (const bool share_first = k_words >= 32; !pair; bn /= 2) {
         const auto few = [&] { return tiles(m_blocks) * split * 2 <= kSms; };
         while ((share_first || bn == 16) && split < kMaxSplit && few() && k_words >= 8 * split) split *= 2;
         if (bn == 16 || !few()) break;
     }
-    const bool four = x_format == LM_MX_E2M1;
     Args a{};
     a.offsets = offsets;
     a.out = out;
