@@ -66,6 +66,7 @@ struct Args {
     void* out;
     int64_t out_stride;
     int rows, groups, n;
+    int x_box, xs_box;  // rows of X and of its scales of a TMA box
     int k_boxes;
     int split;  // CTAs (a cluster) that share a tile's boxes; more than 1: a cluster has one tile
     int out_dtype;
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // In the issuing warps all lanes walk the loop and an elected one issues, so that descriptors and
     // addresses stay in uniform registers (under `if (lane == 0)` a stage took twice as long).
     if (warp == 0) {
-        const uint32_t box_bytes = (FOUR ? kABoxBytes : kABoxBytes / 2) + C::kBBoxBytes;  // spread codes count packed
+        const uint32_t box_bytes = (FOUR ? kABoxBytes : kABoxBytes / 2) + a.x_box * kBoxRow;  // spread codes count packed
         constexpr int kColStep = FOUR ? kBoxRow : C::kBoxCols;  // a box in the map's elements: bytes when packed
         // Narrow tiles are for groups of few rows, whose weights are read once: they leave L2 first
         // (128 tokens over 64 experts: 43.8 -> 41.8 us; with 128 rows a tile it cost 7%).
@@ -368,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!ok) break;
                 if (elect_one()) {
                     uint8_t* dst = smem_s + chunk * C::kScaleBytes;
-                    mbar_arrive_expect_tx(&chunk_full[chunk], C::kScaleBytes);
+                    mbar_arrive_expect_tx(&chunk_full[chunk], (kBlockM + a.xs_box) * C::kChunkBytes);
                     tma_load_2d(dst, &map_ws, &chunk_full[chunk], (box0 + b) * C::kBoxWords * 4, tile.group * a.n + tile.n0);
                     tma_load_2d(dst + kBlockM * C::kChunkBytes, &map_xs, &chunk_full[chunk], (box0 + b) * C::kBoxWords * 4, tile.row0);
                 }
@@ -512,8 +513,13 @@ struct Matrix {
 };
 
 template <int BN, bool PAIR, bool FOUR>
-lm_status launch(const Matrix& w, const Matrix& x, int64_t k, const Args& a, int64_t tiles, cudaStream_t stream) {
+lm_status launch(const Matrix& w, const Matrix& x, int64_t k, Args a, int64_t tiles, cudaStream_t stream) {
     using C = Cfg<BN, PAIR, FOUR>;
+    // No box is higher than X: rows past a map's end cost the TMA more than rows that are there (151552
+    // rows of W by 2048 columns, tiles of 32 rows: 48 us with one row of X in a box of 32).  What a lower
+    // box leaves in shared memory reaches columns of the accumulator that nobody reads.
+    a.x_box = static_cast<int>(std::min<int64_t>(C::kBRows, x.rows));
+    a.xs_box = static_cast<int>(std::min<int64_t>(BN, x.rows));
     CUtensorMap map_w, map_x, map_ws, map_xs;
     const uint64_t cols = static_cast<uint64_t>(mx_padded_cols(k)), pitch = static_cast<uint64_t>(mx_scale_pitch(k));
     const auto encode = [&](const Matrix& m, uint32_t box, uint32_t scale_box, CUtensorMap* codes, CUtensorMap* scales) {
@@ -521,7 +527,7 @@ lm_status launch(const Matrix& w, const Matrix& x, int64_t k, const Args& a, int
         return encode_tensor_map_mx(codes, m.codes, spread, static_cast<uint64_t>(m.rows), FOUR ? cols / 2 : cols, box) &&
                encode_tensor_map_mx_scales(scales, m.scales, static_cast<uint64_t>(m.rows), pitch, scale_box);
     };
-    if (!encode(w, kBlockM, kBlockM, &map_w, &map_ws) || !encode(x, C::kBRows, BN, &map_x, &map_xs)) return context_free_fail(LM_ERR_CUDA, "lm_mx_matmul: cuTensorMapEncodeTiled is unavailable or failed");
+    if (!encode(w, kBlockM, kBlockM, &map_w, &map_ws) || !encode(x, static_cast<uint32_t>(a.x_box), static_cast<uint32_t>(a.xs_box), &map_x, &map_xs)) return context_free_fail(LM_ERR_CUDA, "lm_mx_matmul: cuTensorMapEncodeTiled is unavailable or failed");
     const auto kernel = mx_matmul_kernel<BN, PAIR, FOUR>;
     static std::atomic<uint64_t> configured{0};  // devices whose limit is raised
     if (const cudaError_t e = set_smem_limit_once(kernel, C::kSmemBytes, configured); e != cudaSuccess) return context_free_finish(e);
@@ -575,21 +581,24 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
     const bool four = x_format == LM_MX_E2M1;
     const int64_t each = (rows + groups - 1) / groups;
     int bn = each <= 6 ? 16 : each <= 18 ? 32 : each <= (four ? 64 : 48) ? 64 : 128;
+    if (groups == 1) bn = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : 128;  // not ragged
     const auto tiles = [&](int64_t m_blocks) { return m_blocks * ((rows + bn - 1) / bn + std::min<int64_t>(groups, rows) - 1); };  // at most
     const int64_t m_blocks = (n + kBlockM - 1) / kBlockM, k_words = mx_padded_cols(k) / 128;  // of scales
     if (tiles(m_blocks) > INT32_MAX - kSms) return context_free_fail(LM_ERR_UNSUPPORTED, "lm_mx_matmul: more than 2^31 tiles");
     // Pairs of CTAs where 128 rows a tile give them work (384 rows a group: 195 us without, 170 with).
     const bool pair = bn == 128 && tiles(m_blocks) * 2 > kSms;
     // Fewer tiles than half the SMs: narrower tiles, and clusters of two or four CTAs that share a tile's
-    // columns, at least 512 each, and add their sums through distributed shared memory, without a
+    // columns, at least 512 each (2048 packed), and add their sums through distributed shared memory, without a
     // workspace.  Many columns are shared before tiles get narrower, few after.  (One row, 10944 columns
     // to 2048: one CTA a tile 24 us, two 17, four 12.6; eight, of which not all clusters fit the GPU at
     // once, were slower than four.  128 rows of them: 64 rows a tile shared by four 14 us, 16 rows unshared
-    // 23.  256 rows of 2048 columns: 128 shared by four 10.6, 32 unshared 8.8.)
+    // 23.  256 rows of 2048 columns: 128 shared by four 10.6, 32 unshared 8.8.
+    // Packed: 33 rows of 2048 columns to 1408 unshared 6.4, shared by four 7.4.)
+    const int64_t least = four ? 32 : 8;  // words of columns that two CTAs may share
     int split = 1;
     for (const bool share_first = k_words >= 32; !pair; bn /= 2) {
         const auto few = [&] { return tiles(m_blocks) * split * 2 <= kSms; };
-        while ((share_first || bn == 16) && split < kMaxSplit && few() && k_words >= 8 * split) split *= 2;
+        while ((share_first || bn == 16) && split < kMaxSplit && few() && k_words >= least * split) split *= 2;
         if (bn == 16 || !few()) break;
     }
     Args a{};
