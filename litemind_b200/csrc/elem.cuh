@@ -91,6 +91,11 @@ struct Raw8 {
 
 // ── entry points ─────────────────────────────────────────────────────────
 inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+// Whether two ranges of bytes share one; a null pointer is no range.
+inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x != 0 && y != 0 && x < y + static_cast<uintptr_t>(b_bytes) && y < x + static_cast<uintptr_t>(a_bytes);
+}
 inline int64_t elem_size(int32_t dtype) { return dtype == LM_DTYPE_F32 ? 4 : 2; }
 inline bool is_float_type(int32_t dtype) { return dtype == LM_DTYPE_F32 || dtype == LM_DTYPE_BF16 || dtype == LM_DTYPE_F16; }
 

@@ -313,6 +313,10 @@ lm_status lm_gemm_add_rms_norm_mx(const void* hidden, int32_t dtype, const void*
         !aligned(sum, elem_size(dtype)) || (delta != nullptr && !aligned(delta, elem_size(delta_dtype))) || !aligned(weight, 4) ||
         !aligned(out_bf16, 2) || !aligned(data, 32) || !aligned(scales, 16))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_gemm_add_rms_norm_mx: a null pointer, or data not 32-byte or scales not 16-byte aligned");
+    // Each thread stores the sum over the values it loaded and nobody else's.
+    const int64_t bytes = rows * count * elem_size(dtype), delta_bytes = rows * count * elem_size(delta_dtype);
+    if ((sum != hidden && overlap(sum, bytes, hidden, bytes)) || ((sum != delta || delta_dtype != dtype) && overlap(sum, bytes, delta, delta_bytes)))
+        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_gemm_add_rms_norm_mx: sum overlaps a part of hidden or delta, or a delta of another type");
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     // Rows of a whole number of 16-byte words, all starting on one: eight columns a load.
     const bool vec = count % 8 == 0 && aligned(hidden, 16) && aligned(sum, 16) && aligned(delta, 16) && aligned(out_bf16, 16) && aligned(weight, 16);

@@ -10,6 +10,8 @@
 #include "elem.cuh"
 #include "ptx.cuh"
 
+#include <algorithm>
+
 namespace lm {
 namespace {
 
@@ -340,6 +342,8 @@ lm_status with_parts(int64_t tokens, int64_t parts, F&& f) {
     return context_free_finish(cudaGetLastError());
 }
 
+// Rows that an int32 `at` can name.
+int64_t touched(int64_t n_rows) { return std::min<int64_t>(n_rows, INT32_MAX); }
 bool sizes_ok(int64_t tokens, int32_t k) {
     return tokens >= 0 && k > 0 && k <= LM_SORT_MAX_TOP_K && tokens <= (INT32_MAX - 1024) / k;  // 32-bit pair numbers, with room to step past the last
 }
@@ -413,6 +417,8 @@ lm_status lm_moe_unsort_rows(const void* rows, int32_t dtype, int64_t n_rows, co
     if ((rows == nullptr && n_rows > 0) || at == nullptr || y == nullptr || !aligned(rows, elem_size(dtype)) || !aligned(y, elem_size(y_dtype)) || !aligned(at, 4) ||
         !aligned(weights, 4))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows: a null or misaligned pointer");
+    if (overlap(rows, touched(n_rows) * cols * elem_size(dtype), y, tokens * cols * elem_size(y_dtype)))
+        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows: y overlaps rows");
     const bool vec = cols % 8 == 0 && aligned(rows, 16) && aligned(y, 16);
     lm_status st = LM_OK;
     with_dtype(dtype, [&](auto dt) {
@@ -444,6 +450,9 @@ lm_status lm_moe_unsort_rows_backward(const void* grad_y, const void* rows, int3
         !aligned(grad_y, elem_size(dtype)) || !aligned(rows, elem_size(dtype)) || !aligned(grad_rows, elem_size(dtype)) || !aligned(at, 4) || !aligned(weights, 4) ||
         !aligned(grad_weights, 4))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows_backward: a null or misaligned pointer");
+    const int64_t row_bytes = cols * elem_size(dtype), rows_bytes = touched(n_rows) * row_bytes;
+    if (overlap(grad_y, tokens * row_bytes, grad_rows, rows_bytes) || (grad_rows != rows && overlap(rows, rows_bytes, grad_rows, rows_bytes)))
+        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows_backward: grad_rows overlaps grad_y or part of rows");
     const bool vec = cols % 8 == 0 && aligned(grad_y, 16) && aligned(rows, 16) && aligned(grad_rows, 16);
     with_dtype(dtype, [&](auto dt) {
         with_bool(vec, [&](auto v) {

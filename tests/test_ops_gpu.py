@@ -206,6 +206,23 @@ def test_product_long_columns(rows, k):
             check_product(ops.mx_matmul(x, w, offsets, dtype=dtype), x, w, cut, k, dtype)
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("counts", [[1], [7], [17], [31], [33], [60], [65], [100], [129], [1, 0, 6], [50, 49], [3, 60, 1]])
+def test_product_few_rows_after_nan(counts, fmt):
+    """Fewer rows than a tile has room for, in every CTA: what an earlier product left in shared memory
+    and TMEM, NaN here, reaches nothing.  Also packed rows of many columns, shared by a cluster."""
+    n, k = 148 * 128 // len(counts), 640
+    x, w, offsets, cut = product_inputs(sum(counts), counts, n, k, fmt)
+    nan = ops.MxTensor(torch.full((300, x.data.shape[1]), 0x7F, dtype=torch.uint8, device="cuda"), torch.full((300, x.scales.shape[1]), 255, dtype=torch.uint8, device="cuda"),
+                       k, fmt)
+    flat = ops.MxTensor(w.data.view(-1, w.data.shape[-1]), w.scales.view(-1, w.scales.shape[-1]), k, "e2m1")
+    for rows in (16, 32, 64, 300):
+        assert torch.isnan(ops.mx_matmul(ops.MxTensor(nan.data[:rows], nan.scales[:rows], k, fmt), flat, dtype=F32)).all()
+        check_product(ops.mx_matmul(x, w, offsets, dtype=F32), x, w, cut, k, F32)
+    x, w, offsets, cut = product_inputs(7, counts, 130, 6000, fmt)
+    check_product(ops.mx_matmul(x, w, offsets, dtype=BF16), x, w, cut, 6000, BF16)
+
+
 def test_product_leaves_other_rows_and_columns():
     """Rows of no group, and the columns between n and a wider output's stride, keep their values."""
     x, w, offsets, cut = product_inputs(1, [3, 0, 40], 70, 200, "e4m3", extra=9)

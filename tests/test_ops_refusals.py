@@ -87,6 +87,16 @@ def test_sort(lib):
     empty(lib, "lm_moe_unsort_rows_backward", good, tokens=[0])
 
 
+def test_overlaps(lib):
+    at, far = 1 << 30, 1 << 32
+    back = dict(rows=P, dtype=BF16, n_rows=6, at=at, weights=at, tokens=3, k=2, cols=64, y=far, y_dtype=BF16, accumulate=0)
+    refused(lib, "lm_moe_unsort_rows", back, y=[P, P + 6 * 128 - 2, P - 3 * 128 + 2])
+    grad = dict(grad_y=P, rows=far, dtype=BF16, n_rows=6, at=at, weights=at, tokens=3, k=2, cols=64, grad_rows=far, grad_weights=at)
+    refused(lib, "lm_moe_unsort_rows_backward", grad, grad_rows=[P, P + 3 * 128 - 16, far + 128, far - 6 * 128 + 16])
+    norm = dict(hidden=P, dtype=F32, delta=far, ddtype=BF16, weight=at, rows=4, count=64, eps=1e-6, sum=2 * far, bf16=None, fmt=E4M3, data=at, scales=at)
+    refused(lib, "lm_gemm_add_rms_norm_mx", norm, sum=[P + 256, P - 256, far, far + 4 * 128 - 16])
+
+
 def test_cpp_forms(tmp_path):
     """Mx.hpp and TokenSort.hpp compile as a user compiles them and answer as the C entries do."""
     from tests.test_cpp_mirror import _compile
