@@ -241,8 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int m_blocks = (a.n + kBlockM * C::kCtas - 1) / (kBlockM * C::kCtas);
     const int total = s_tiles[a.groups] * m_blocks;
 
-    // In the issuing warps all lanes walk the loop and an elected one issues, so that descriptors and
-    // addresses stay in uniform registers (under `if (lane == 0)` a stage took twice as long).
+    // An elected lane issues, so that descriptors and addresses stay in uniform registers (under
+    // `if (lane == 0)` a stage took twice as long).
     if (warp == 0) {
         const uint32_t box_bytes = (FOUR ? kABoxBytes : kABoxBytes / 2) + a.x_box * kBoxRow;  // spread codes count packed
         constexpr int kColStep = FOUR ? kBoxRow : C::kBoxCols;  // a box in the map's elements: bytes when packed
@@ -285,41 +285,42 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = 0; i < S; ++i)
                 if (issued & (1u << i)) mbar_wait_drain(&full[i], (issued_phase >> i) & 1u, 100000000ull);
     } else if (warp == 1 && rank == 0) {
-        int stage = 0, sg = 0, acc = 0;
-        uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
-        bool ok = true, any = false, seen = false, sf_seen = false;
-        const uint64_t desc_a = umma_desc_sw128(smem_u32(smem_a)), desc_b = umma_desc_sw128(smem_u32(smem_b));
-        constexpr int U = C::kRound;
-        const auto after = [](int st, int by) { return st + by >= S ? st + by - S : st + by; };
-        for (int t = first; ok && t < total; t += step) {
-            int width = BN;  // a pair's MMAs are no wider than the tile's rows need; one CTA's take 50 cycles at least
-            if constexpr (PAIR) width = mma_n<PAIR>(tile_at<BN, PAIR, FOUR>(a, s_cut, s_tiles, t, m_blocks, rank).rows);
-            const uint32_t shape = static_cast<uint32_t>(width >> 3) << 17;
-            ok = __all_sync(0xffffffffu, wait(&tmem_empty[acc], acc_phase ^ 1u, kDevTimeoutMma));
-            const uint32_t d = tmem + acc * BN;
-            for (int b = 0; ok && b < boxes; b += U * B) {
-                const int stages = min(U, (boxes - b + B - 1) / B);
-                const bool sf_begin = b % C::kChunkBoxes == 0;
-                if ((sf_begin && !sf_seen) || !seen) {
-                    ok = !sf_begin || sf_seen || wait(&sf_full[sg], sf_phase, kDevTimeoutMma);
+        // One lane does all of it: the votes and elections of a whole warp cost more than they order
+        // (64 experts of 12 rows: 40.1 us, one lane 39.2; 384 rows a group 173 and 162).
+        if (elect_one()) {
+            int stage = 0, sg = 0, acc = 0;
+            uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
+            bool ok = true, any = false, seen = false, sf_seen = false;
+            const uint64_t desc_a = umma_desc_sw128(smem_u32(smem_a)), desc_b = umma_desc_sw128(smem_u32(smem_b));
+            constexpr int U = C::kRound;
+            const auto after = [](int st, int by) { return st + by >= S ? st + by - S : st + by; };
+            for (int t = first; ok && t < total; t += step) {
+                int width = BN;  // a pair's MMAs are no wider than the tile's rows need; one CTA's take 50 cycles at least
+                if constexpr (PAIR) width = mma_n<PAIR>(tile_at<BN, PAIR, FOUR>(a, s_cut, s_tiles, t, m_blocks, rank).rows);
+                const uint32_t shape = static_cast<uint32_t>(width >> 3) << 17;
+                ok = wait(&tmem_empty[acc], acc_phase ^ 1u, kDevTimeoutMma);
+                const uint32_t d = tmem + acc * BN;
+                for (int b = 0; ok && b < boxes; b += U * B) {
+                    const int stages = min(U, (boxes - b + B - 1) / B);
+                    const bool sf_begin = b % C::kChunkBoxes == 0;
+                    if ((sf_begin && !sf_seen) || !seen) {
+                        ok = !sf_begin || sf_seen || wait(&sf_full[sg], sf_phase, kDevTimeoutMma);
 #pragma unroll
-                    for (int u = 0; u < U; ++u)
-                        if (u < stages) ok = ok && wait(&full[after(stage, u)], phase ^ (stage + u >= S), kDevTimeoutMma);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                }
-                tc_fence_after();
-                const bool last = b + stages * B >= boxes;
-                const bool sf_end = last || (b + stages * B) % C::kChunkBoxes == 0;
-                const int next = after(stage, stages), sg_next = sg + 1 == G ? 0 : sg + 1;
-                const uint32_t next_phase = phase ^ (stage + stages >= S);
-                // A look at the next round while the tensor cores still work: even the wait for a
-                // complete barrier costs as much as an MMA.
-                bool look = true;
+                        for (int u = 0; u < U; ++u)
+                            if (u < stages) ok = ok && wait(&full[after(stage, u)], phase ^ (stage + u >= S), kDevTimeoutMma);
+                        if (!ok) break;
+                    }
+                    tc_fence_after();
+                    const bool last = b + stages * B >= boxes;
+                    const bool sf_end = last || (b + stages * B) % C::kChunkBoxes == 0;
+                    const int next = after(stage, stages), sg_next = sg + 1 == G ? 0 : sg + 1;
+                    const uint32_t next_phase = phase ^ (stage + stages >= S);
+                    // A look at the next round while the tensor cores still work: even the wait for a
+                    // complete barrier costs as much as an MMA.
+                    bool look = true;
 #pragma unroll
-                for (int u = 0; u < U; ++u) look = look && mbar_test(&full[after(next, u)], next_phase ^ (next + u >= S));
-                const bool sf_look = sf_end && mbar_test(&sf_full[sg_next], sf_phase ^ (sg_next == 0));
-                if (elect_one()) {
+                    for (int u = 0; u < U; ++u) look = look && mbar_test(&full[after(next, u)], next_phase ^ (next + u >= S));
+                    const bool sf_look = sf_end && mbar_test(&sf_full[sg_next], sf_phase ^ (sg_next == 0));
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
                         if (u >= stages) break;
@@ -344,20 +345,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (sf_end) commit(&sf_empty[sg]);
                     if (last) commit(&tmem_full[acc]);
+                    any = true;
+                    seen = look;
+                    phase = next_phase, stage = next;
+                    if (sf_end) sf_seen = sf_look, sf_phase ^= sg_next == 0, sg = sg_next;
                 }
-                __syncwarp();
-                any = true;
-                seen = __all_sync(0xffffffffu, look);
-                phase = next_phase, stage = next;
-                if (sf_end) sf_seen = __all_sync(0xffffffffu, sf_look), sf_phase ^= sg_next == 0, sg = sg_next;
+                if (++acc == 2) acc = 0, acc_phase ^= 1u;
             }
-            if (++acc == 2) acc = 0, acc_phase ^= 1u;
+            if (!ok && any) {  // the MMAs issued so far end before TMEM is released
+                commit(&drain);
+                mbar_wait_drain(&drain, 0, 100000000ull);
+            }
         }
-        if (!ok && any) {  // the MMAs issued so far end before TMEM is released
-            if (elect_one()) commit(&drain);
-            __syncwarp();
-            mbar_wait_drain(&drain, 0, 100000000ull);
-        }
+        __syncwarp();
     } else if (warp == 2) {
         int chunk = 0;
         uint32_t phase = 0, issued = 0, issued_phase = 0;
