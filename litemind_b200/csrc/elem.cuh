@@ -73,13 +73,18 @@ __device__ __forceinline__ void store8(typename Elem<DT>::T* p, const float (&v)
 // while loads are in flight.
 template <int DT>
 struct Raw8 {
-    uint32_t w[2 * sizeof(typename Elem<DT>::T)];
+    alignas(16) uint32_t w[2 * sizeof(typename Elem<DT>::T)];
     __device__ __forceinline__ void load(const typename Elem<DT>::T* p) {
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(w) / 16); ++i) {
             const uint4 q = reinterpret_cast<const uint4*>(p)[i];
             w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
         }
+    }
+    __device__ __forceinline__ void narrow(const float (&v)[8]) { store8<DT>(reinterpret_cast<typename Elem<DT>::T*>(w), v); }
+    __device__ __forceinline__ void store(typename Elem<DT>::T* p) const {
+#pragma unroll
+        for (int i = 0; i < static_cast<int>(sizeof(w) / 16); ++i) reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
     }
     __device__ __forceinline__ void widen(float (&v)[8]) const {
         typename Elem<DT>::T e[8];

@@ -153,12 +153,17 @@ __device__ __forceinline__ void load_pair(const typename Elem<DT>::T* hidden, co
 template <int DT, bool VEC>
 __device__ __forceinline__ double add_store(float (&v)[8], const float (&d)[8], bool add, int64_t col, int64_t cols, typename Elem<DT>::T* sum) {
     double s = 0.0;
+    if (add) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (add) v[i] = Elem<DT>::widen(Elem<DT>::narrow(v[i] + d[i]));
-        s = fma(static_cast<double>(v[i]), static_cast<double>(v[i]), s);
+        for (int i = 0; i < 8; ++i) v[i] += d[i];
     }
-    store_cols<DT, VEC>(sum, col, cols, v);
+    Raw8<DT> r;  // rounded once, for the store and the norm
+    r.narrow(v);
+    r.widen(v);
+    if (VEC && col + 8 <= cols) r.store(sum + col);
+    else store_cols<DT, false>(sum, col, cols, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = fma(static_cast<double>(v[i]), static_cast<double>(v[i]), s);
     return s;
 }
 
@@ -169,7 +174,12 @@ __device__ __forceinline__ void put_norm(float (&v)[8], float inverse, const flo
     float g[8];
     load_cols<LM_DTYPE_F32, VEC>(weight, col, cols, g);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? v[i] * inverse * g[i] : 0.0f;
+    for (int i = 0; i < 8; ++i) v[i] = v[i] * inverse * g[i];
+    if (VEC ? col >= cols : col + 8 > cols) {  // an infinite inverse leaves NaN past the row's end
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (VEC || col + i >= cols) v[i] = 0.0f;
+    }
     if (out_bf16 != nullptr) store_cols<LM_DTYPE_BF16, VEC>(out_bf16, col, cols, v);
     uint32_t byte;
     if (format == LM_MX_E2M1) {
@@ -182,17 +192,25 @@ __device__ __forceinline__ void put_norm(float (&v)[8], float inverse, const flo
     if ((threadIdx.x & 3) == 0) scales[col / kMxBlock] = static_cast<uint8_t>(byte);
 }
 
-// The sum of s over the CTA.
+// The inverse root of the CTA's mean square: its first warp's work, 15% of the instructions of a row
+// of 2048 when every thread did it.
 template <int T>
-__device__ __forceinline__ double block_sum(double s) {
-    __shared__ double red[T / 32];
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
-    __syncthreads();
-    s = 0.0;
+__device__ __forceinline__ float block_inverse(double s, double inv_cols, double eps) {
+    __shared__ double red[32];
+    __shared__ float inverse;
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < T / 32; ++i) s += red[i];
-    return s;
+    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    if (lane == 0) red[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        s = lane < T / 32 ? red[lane] : 0.0;
+#pragma unroll
+        for (int off = T / 64 > 8 ? 16 : T / 64 > 4 ? 8 : 4; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        if (lane == 0) inverse = static_cast<float>(rsqrt(s * inv_cols + eps));
+    }
+    __syncthreads();
+    return inverse;
 }
 
 // A CTA of T threads a row, eight columns a thread of every stretch of 8 T.  With CHUNKS > 0 that
@@ -217,7 +235,7 @@ __global__ void __launch_bounds__(T)
         for (int c = 0; c < CHUNKS; ++c) load_pair<DT, VEC>(hidden, delta, delta_f32 != 0, first + c * T * 8, cols, v[c], d[c]);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) s += add_store<DT, VEC>(v[c], d[c], delta != nullptr, first + c * T * 8, cols, sum);
-        const float inverse = static_cast<float>(rsqrt(block_sum<T>(s) * inv_cols + eps));
+        const float inverse = block_inverse<T>(s, inv_cols, eps);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c)
             if (first + c * T * 8 < end) put_norm<VEC>(v[c], inverse, weight, first + c * T * 8, cols, out_bf16, format, data, data_pitch, scales);
@@ -227,7 +245,7 @@ __global__ void __launch_bounds__(T)
             load_pair<DT, VEC>(hidden, delta, delta_f32 != 0, col, cols, v, d);
             s += add_store<DT, VEC>(v, d, delta != nullptr, col, cols, sum);
         }
-        const float inverse = static_cast<float>(rsqrt(block_sum<T>(s) * inv_cols + eps));
+        const float inverse = block_inverse<T>(s, inv_cols, eps);
         for (int64_t col = first; col < end; col += T * 8) {
             load_cols<DT, VEC>(sum, col, cols, v);
             put_norm<VEC>(v, inverse, weight, col, cols, out_bf16, format, data, data_pitch, scales);
