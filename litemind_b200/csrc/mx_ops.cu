@@ -135,25 +135,45 @@ __global__ void __launch_bounds__(kThreads)
     }
 }
 
-// Eight values of the residual and of its update; zeros for an update that is not there.
-template <int DT, bool VEC>
-__device__ __forceinline__ void load_pair(const typename Elem<DT>::T* hidden, const void* delta, bool delta_f32, int64_t col, int64_t cols, float (&v)[8],
-                                          float (&d)[8]) {
-    load_cols<DT, VEC>(hidden, col, cols, v);
-    if (delta == nullptr) {
+// Eight columns of the residual and of its update as they lie in memory, so that the loads of both
+// and of every stretch are in flight together: whatever converts the first of them waits for it.
+template <int DT>
+struct Pair8 {
+    Raw8<DT> hidden;
+    Raw8<LM_DTYPE_F32> delta;  // bf16: in the first half
+};
+template <int DT, bool VEC, int N>
+__device__ __forceinline__ void load_pairs(const typename Elem<DT>::T* hidden, const void* delta, bool delta_f32, int64_t col, int64_t step, int64_t cols,
+                                           Pair8<DT> (&p)[N]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = 0.0f;
-    } else if (delta_f32) {
-        load_cols<LM_DTYPE_F32, VEC>(static_cast<const float*>(delta), col, cols, d);
+    for (int c = 0; c < N; ++c) p[c].hidden = load_raw<DT, VEC>(hidden, col + c * step, cols);
+    if (delta == nullptr) return;
+    if (delta_f32) {
+#pragma unroll
+        for (int c = 0; c < N; ++c) p[c].delta = load_raw<LM_DTYPE_F32, VEC>(static_cast<const float*>(delta), col + c * step, cols);
     } else {
-        load_cols<LM_DTYPE_BF16, VEC>(static_cast<const __nv_bfloat16*>(delta), col, cols, d);
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+            const Raw8<LM_DTYPE_BF16> d = load_raw<LM_DTYPE_BF16, VEC>(static_cast<const __nv_bfloat16*>(delta), col + c * step, cols);
+            memcpy(p[c].delta.w, d.w, sizeof d.w);
+        }
     }
 }
 // Their sum, rounded to the residual's type and stored, in v; returns the sum of its squares.
 template <int DT, bool VEC>
-__device__ __forceinline__ double add_store(float (&v)[8], const float (&d)[8], bool add, int64_t col, int64_t cols, typename Elem<DT>::T* sum) {
+__device__ __forceinline__ double add_store(const Pair8<DT>& p, bool add, bool delta_f32, float (&v)[8], int64_t col, int64_t cols,
+                                            typename Elem<DT>::T* sum) {
     double s = 0.0;
+    p.hidden.widen(v);
     if (add) {
+        float d[8];
+        if (delta_f32) {
+            p.delta.widen(d);
+        } else {
+            Raw8<LM_DTYPE_BF16> half;
+            memcpy(half.w, p.delta.w, sizeof half.w);
+            half.widen(d);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] += d[i];
     }
@@ -214,13 +234,14 @@ __device__ __forceinline__ float block_inverse(double s, double inv_cols, double
 }
 
 // A CTA of T threads a row, eight columns a thread of every stretch of 8 T.  With CHUNKS > 0 that
-// many stretches are loaded before anything is stored (sum may be hidden or delta, so the compiler
-// cannot), and stay in registers between the sum and the norm; CHUNKS = 0 reads the stored sum again
-// (each thread its own stores).  The sum is normalised as stored, its squares added in f64 as
-// lm_gemm_rms_norm adds them.  Instructions bound it for 16-bit rows (f64 square root and division
-// in every thread took 62 us at 16384 x 2048, rsqrt 52) and HBM for f32 rows.
+// many stretches are loaded before anything is converted or stored (sum may be hidden or delta, so
+// the compiler cannot), and stay in registers between the sum and the norm; CHUNKS = 0 reads the
+// stored sum again (each thread its own stores).  The sum is normalised as stored, its squares added
+// in f64 as lm_gemm_rms_norm adds them.  bf16 rows: 16384 x 2048 in 44 us, 5.4 TB/s, of which
+// instructions take most (issue slots 77% busy at 49 us; with loads converted one after another two
+// stretches took 56 us, with 48 registers a thread 47); f32 rows: 65 us, HBM's rate.
 template <int DT, bool VEC, int T, int CHUNKS>
-__global__ void __launch_bounds__(T)
+__global__ void __launch_bounds__(T, VEC && CHUNKS != 1 ? 1536 / T : 1)
     add_rms_norm_mx_kernel(const typename Elem<DT>::T* hidden, const void* delta, int delta_f32, const float* __restrict__ weight, int64_t cols,
                            double inv_cols, double eps, typename Elem<DT>::T* sum, __nv_bfloat16* __restrict__ out_bf16, int format,
                            uint8_t* __restrict__ data, int64_t data_pitch, uint8_t* __restrict__ scales, int64_t scale_pitch) {
@@ -230,20 +251,21 @@ __global__ void __launch_bounds__(T)
     if (out_bf16 != nullptr) out_bf16 += row * cols;
     double s = 0.0;
     if constexpr (CHUNKS > 0) {
-        float v[CHUNKS][8], d[CHUNKS][8];
+        Pair8<DT> p[CHUNKS];
+        float v[CHUNKS][8];
+        load_pairs<DT, VEC>(hidden, delta, delta_f32 != 0, first, T * 8, cols, p);
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) load_pair<DT, VEC>(hidden, delta, delta_f32 != 0, first + c * T * 8, cols, v[c], d[c]);
-#pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) s += add_store<DT, VEC>(v[c], d[c], delta != nullptr, first + c * T * 8, cols, sum);
+        for (int c = 0; c < CHUNKS; ++c) s += add_store<DT, VEC>(p[c], delta != nullptr, delta_f32 != 0, v[c], first + c * T * 8, cols, sum);
         const float inverse = block_inverse<T>(s, inv_cols, eps);
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c)
             if (first + c * T * 8 < end) put_norm<VEC>(v[c], inverse, weight, first + c * T * 8, cols, out_bf16, format, data, data_pitch, scales);
     } else {
-        float v[8], d[8];
+        float v[8];
         for (int64_t col = first; col < cols; col += T * 8) {
-            load_pair<DT, VEC>(hidden, delta, delta_f32 != 0, col, cols, v, d);
-            s += add_store<DT, VEC>(v, d, delta != nullptr, col, cols, sum);
+            Pair8<DT> p[1];
+            load_pairs<DT, VEC>(hidden, delta, delta_f32 != 0, col, 0, cols, p);
+            s += add_store<DT, VEC>(p[0], delta != nullptr, delta_f32 != 0, v, col, cols, sum);
         }
         const float inverse = block_inverse<T>(s, inv_cols, eps);
         for (int64_t col = first; col < end; col += T * 8) {
@@ -350,20 +372,30 @@ lm_status lm_gemm_add_rms_norm_mx(const void* hidden, int32_t dtype, const void*
                     static_cast<const T*>(hidden), delta, delta_dtype == LM_DTYPE_F32, weight, count, 1.0 / static_cast<double>(count), epsilon, static_cast<T*>(sum),
                     reinterpret_cast<__nv_bfloat16*>(out_bf16), format, data, mx_data_pitch(format, count), scales, mx_scale_pitch(count));
             };
-            // Few idle threads, then several CTAs an SM: bf16 rows of 1024 took 31 us with 128 threads and
-            // 49 with 256 (20000 rows), of 6144 52 with 384 and 65 with 1024 (4096 rows), and f32 rows of
-            // 8192 138 with 512 and 157 with 1024 (8192 rows).  Two stretches a thread lost where one of
-            // 512 threads covers the row (60 us, 57 at 8192 x 4096).
-            using std::integral_constant;
-            const integral_constant<int, 1> one;
-            const integral_constant<int, 2> two;
-            if (wide <= 1024) go(integral_constant<int, 128>{}, one);
-            else if (wide <= 2048) go(integral_constant<int, 256>{}, one);
-            else if (wide <= 4096) go(integral_constant<int, 512>{}, one);
-            else if (wide <= 6144) go(integral_constant<int, 384>{}, two);
-            else if (wide <= 8192) go(integral_constant<int, 512>{}, two);
-            else if (wide <= 16384) go(integral_constant<int, 1024>{}, two);
-            else go(integral_constant<int, 512>{}, integral_constant<int, 0>{});
+            // T threads for every eight of the widest row of a class (bf16 rows of 1024 took 31 us with 128
+            // threads and 49 with 256, 20000 rows).  bf16 rows that fill the GPU three times over, which
+            // instructions bound, take two stretches a thread (us, two and one: 16384 x 2048 44 and 49, 4096 x
+            // 8192 49 and 56, 4000 x 2048 12.8 and 13.3); fewer rows, where latency counts, and f32 rows,
+            // which HBM bounds, take one (2000 x 2048 7.2 and 6.5, 8192 x 8192 f32 136 and 132).  Wider
+            // rows read their sum again (2048 x 16384: 63, held in registers 80).
+            const bool many = rows * wide > int64_t(3) * 148 * 2048 * 8;
+            const auto fit = [&](auto stretches) {
+                constexpr int C = decltype(stretches)::value;
+                if (wide <= 1024) go(std::integral_constant<int, 128 / C>{}, stretches);
+                else if (wide <= 2048) go(std::integral_constant<int, 256 / C>{}, stretches);
+                else if (wide <= 4096) go(std::integral_constant<int, 512 / C>{}, stretches);
+                else if (wide <= 6144) go(std::integral_constant<int, 768 / C>{}, stretches);
+                else go(std::integral_constant<int, 1024 / C>{}, stretches);
+            };
+            if (wide > 8192) {
+                if (many) go(std::integral_constant<int, 512>{}, std::integral_constant<int, 0>{});
+                else go(std::integral_constant<int, 1024>{}, std::integral_constant<int, 0>{});
+            } else if constexpr (DT == LM_DTYPE_BF16) {
+                if (many) fit(std::integral_constant<int, 2>{});
+                else fit(std::integral_constant<int, 1>{});
+            } else {
+                fit(std::integral_constant<int, 1>{});
+            }
         });
     });
     return context_free_finish(cudaGetLastError());

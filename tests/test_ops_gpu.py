@@ -334,6 +334,13 @@ def test_add_rms_norm(rows, cols, dtype, ddtype, fmt):
     assert again[2] is None and torch.equal(again[1].data, q.data) and torch.equal(again[1].scales, q.scales)
 
 
+@pytest.mark.parametrize("dtype,ddtype", [(F32, BF16), (BF16, F32), (BF16, BF16), (BF16, None)])
+@pytest.mark.parametrize("rows,cols", [(15000, 500), (7200, 1017), (3700, 2048), (1900, 4000), (1300, 6144), (1250, 5001), (1000, 8192), (800, 9999), (600, 16384)])
+def test_add_rms_norm_many_rows(rows, cols, dtype, ddtype):
+    """Rows that fill the GPU several times over, of every class of widths."""
+    test_add_rms_norm(rows, cols, dtype, ddtype, "e4m3")
+
+
 def test_add_rms_norm_in_place_and_special_rows():
     g = gen(2)
     hidden, delta, weight = normal(g, 4, 300), normal(g, 4, 300), normal(g, 300)
