@@ -455,6 +455,27 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
  * (lm_mx_matmul) on the current device since the last call, then clears it, as lm_moe_sync does for a context: LM_ERR_DEVICE_TIMEOUT, and the results of
  * the calls since then are invalid. */
 lm_status lm_ops_sync(void* stream);
+/*
+ * Testing hooks of that path, for the whole process; production code leaves them at 0.
+ *   LM_DEBUG_PRODUCT_STALL  a LM_STALL_* barrier of lm_mx_matmul's pipeline that expects one arrival
+ *                           more than it gets, in the launches (and captures) that follow: waits on
+ *                           it run out, the kernel lets its copies and MMAs end and returns, and
+ *                           lm_ops_sync reports LM_ERR_DEVICE_TIMEOUT
+ *   LM_DEBUG_WAIT_LIMIT_NS  bound of each of the product's waits in ns (0: 2 s, also the maximum)
+ * No GPU fault is involved: the kernel only stops waiting.
+ */
+enum { LM_DEBUG_PRODUCT_STALL = 3 };
+enum {
+    LM_STALL_FULL = 1,     /* a stage's copies */
+    LM_STALL_EMPTY,        /* its slot free again */
+    LM_STALL_CHUNK_FULL,   /* a chunk of scales in shared memory */
+    LM_STALL_CHUNK_EMPTY,
+    LM_STALL_SCALE_FULL,   /* scales in TMEM */
+    LM_STALL_SCALE_EMPTY,
+    LM_STALL_TMEM_FULL,    /* an accumulator */
+    LM_STALL_TMEM_EMPTY
+};
+lm_status lm_ops_debug_set(int32_t knob, int64_t value);
 
 /* ── gemm:: kernels on device memory (include/Gemm.hpp:23-72) ──────────────── */
 

@@ -34,6 +34,9 @@ LM_TOPK_GREEDY = 0
 LM_TOPK_GROUP_LIMITED_GREEDY = 1
 LM_DEBUG_GRID_EXTRA = 1
 LM_DEBUG_WAIT_LIMIT_NS = 2
+LM_DEBUG_PRODUCT_STALL = 3
+(LM_STALL_FULL, LM_STALL_EMPTY, LM_STALL_CHUNK_FULL, LM_STALL_CHUNK_EMPTY, LM_STALL_SCALE_FULL, LM_STALL_SCALE_EMPTY,
+ LM_STALL_TMEM_FULL, LM_STALL_TMEM_EMPTY) = range(1, 9)
 
 # Every symbol include/litemind_moe.h declares, with (restype, argtypes).
 _vp, _i32, _i64, _f32, _u64p = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.POINTER(C.c_uint64)
@@ -104,6 +107,7 @@ SIGNATURES = {
     "lm_mx_dequantize": (_i32, [_vp, _vp, _i32, _i64, _i64, _vp, _i32, _i64, _vp]),
     "lm_mx_matmul": (_i32, [_vp, _vp, _i32, _i64, _vp, _vp, _i32, _i64, _i64, _vp, _vp, _i32, _i64, _vp]),
     "lm_ops_sync": (_i32, [_vp]),
+    "lm_ops_debug_set": (_i32, [_i32, _i64]),
     "lm_gemm_add_rms_norm_mx": (_i32, [_vp, _i32, _vp, _i32, _vp, _i64, _i64, _f32, _vp, _vp, _i32, _vp, _vp, _vp]),
     "lm_kernel_description": (C.c_char_p, []),
     "lm_gemm_matvec_bf16": (_i32, [_vp, _vp, _vp, _i64, _i64, _vp]),

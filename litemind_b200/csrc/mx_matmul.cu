@@ -20,12 +20,15 @@
 //   8-15   epilogue: TMEM to registers to out, rounded once; two warps a quadrant share the rows of X
 // A stage costs the issuer about 400 cycles of waits, descriptors and commits whatever its width,
 // and the four MMAs of a box take 200 (N = 16) to 256 (N = 128): hence two boxes a stage.
-// Every wait is bounded (ptx.cuh): a pipeline that stalls records a status for lm_ops_sync.
+// Every wait is bounded (ptx.cuh): a pipeline that stalls records a status for lm_ops_sync.  Once all
+// warps have stopped, each waits for what it left in flight (copies, MMAs) before shared memory and
+// TMEM are given up; a pair does so together, since the second CTA's copies end on the first's barriers.
 #include "moe_internal.h"
 #include "mx_block.cuh"
 #include "ptx.cuh"
 
 #include <algorithm>
+#include <atomic>
 
 namespace lm {
 namespace {
@@ -71,6 +74,8 @@ struct Args {
     int split;  // CTAs (a cluster) that share a tile's boxes; more than 1: a cluster has one tile
     int out_dtype;
     int out_pairs;  // 16-bit elements n, n + 1 (n even) lie on 4-byte boundaries
+    int stall;      // testing only: a LM_STALL_* barrier that expects one arrival more than it gets
+    uint64_t wait_limit_ns;
     int* status;
 };
 
@@ -183,6 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __shared__ uint64_t full[S], empty[S], chunk_full[C::kChunks], chunk_empty[C::kChunks], sf_full[G], sf_empty[G], tmem_full[2], tmem_empty[2], drain;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort;
+    __shared__ uint32_t s_peer_gave_up, s_peer_sent;  // written by the pair's other CTA
     uint8_t* smem_a = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* smem_b = smem_a + S * B * kABoxBytes;
     uint8_t* smem_s = smem_b + S * B * C::kBBoxBytes;  // chunks: 128 rows of W's scales, then BN of X's
@@ -197,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int units = (a.k_boxes + kUnit - 1) / kUnit, box0 = units * part / split * kUnit, boxes = min(a.k_boxes, units * (part + 1) / split * kUnit) - box0;
 
     const auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-        return mbar_wait(bar, parity, abort_flag, a.status, code);
+        return mbar_wait(bar, parity, abort_flag, a.status, code, a.wait_limit_ns);
     };
     const auto commit = [&](uint64_t* bar) {
         if constexpr (PAIR) umma_commit_both(bar);
@@ -213,12 +219,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_prefetch_desc(&map_x);
         tma_prefetch_desc(&map_ws);
         tma_prefetch_desc(&map_xs);
-        for (int i = 0; i < S; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
-        for (int i = 0; i < C::kChunks; ++i) mbar_init(&chunk_full[i], 1), mbar_init(&chunk_empty[i], 4);
-        for (int i = 0; i < G; ++i) mbar_init(&sf_full[i], 4 * C::kCtas), mbar_init(&sf_empty[i], 1);
-        for (int i = 0; i < 2; ++i) mbar_init(&tmem_full[i], 1), mbar_init(&tmem_empty[i], 8 * C::kCtas);
+        const auto init = [&](uint64_t* bars, int count, uint32_t arrivals, int stall) {
+            for (int i = 0; i < count; ++i) mbar_init(&bars[i], arrivals + (a.stall == stall));
+        };
+        init(full, S, 1, LM_STALL_FULL), init(empty, S, 1, LM_STALL_EMPTY);
+        init(chunk_full, C::kChunks, 1, LM_STALL_CHUNK_FULL), init(chunk_empty, C::kChunks, 4, LM_STALL_CHUNK_EMPTY);
+        init(sf_full, G, 4 * C::kCtas, LM_STALL_SCALE_FULL), init(sf_empty, G, 1, LM_STALL_SCALE_EMPTY);
+        init(tmem_full, 2, 1, LM_STALL_TMEM_FULL), init(tmem_empty, 2, 8 * C::kCtas, LM_STALL_TMEM_EMPTY);
         mbar_init(&drain, 1);
-        s_abort = 0;
+        s_abort = 0, s_peer_gave_up = 0, s_peer_sent = 0;
         fence_mbar_init();
     }
     __syncwarp();
@@ -241,16 +250,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int m_blocks = (a.n + kBlockM * C::kCtas - 1) / (kBlockM * C::kCtas);
     const int total = s_tiles[a.groups] * m_blocks;
 
+    const uint32_t box_bytes = (FOUR ? kABoxBytes : kABoxBytes / 2) + a.x_box * kBoxRow;  // spread codes count packed
+    // What a thread may leave in flight: stages sent (warp 0), chunks sent (warp 2), MMAs (the issuing lane).
+    uint32_t sent = 0;
+    bool mmas = false;
+
     // An elected lane issues, so that descriptors and addresses stay in uniform registers (under
     // `if (lane == 0)` a stage took twice as long).
     if (warp == 0) {
-        const uint32_t box_bytes = (FOUR ? kABoxBytes : kABoxBytes / 2) + a.x_box * kBoxRow;  // spread codes count packed
         constexpr int kColStep = FOUR ? kBoxRow : C::kBoxCols;  // a box in the map's elements: bytes when packed
         // Narrow tiles are for groups of few rows, whose weights are read once: they leave L2 first
         // (128 tokens over 64 experts: 43.8 -> 41.8 us; with 128 rows a tile it cost 7%).
         const uint64_t once = policy_evict_first();
         int stage = 0;
-        uint32_t phase = 0, issued = 0, issued_phase = 0;
+        uint32_t phase = 0;
         bool ok = true;
         for (int t = first; ok && t < total; t += step) {
             const Tile tile = tile_at<BN, PAIR, FOUR>(a, s_cut, s_tiles, t, m_blocks, rank);
@@ -276,21 +289,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
                 __syncwarp();
-                issued |= 1u << stage;
-                issued_phase = (issued_phase & ~(1u << stage)) | (phase << stage);
+                ++sent;
                 if (++stage == S) stage = 0, phase ^= 1u;
             }
         }
-        if (!ok && rank == 0)  // copies in flight land before shared memory is given up
-            for (int i = 0; i < S; ++i)
-                if (issued & (1u << i)) mbar_wait_drain(&full[i], (issued_phase >> i) & 1u, 100000000ull);
     } else if (warp == 1 && rank == 0) {
         // One lane does all of it: the votes and elections of a whole warp cost more than they order
         // (64 experts of 12 rows: 40.1 us, one lane 39.2; 384 rows a group 173 and 162).
         if (elect_one()) {
             int stage = 0, sg = 0, acc = 0;
             uint32_t phase = 0, sf_phase = 0, acc_phase = 0;
-            bool ok = true, any = false, seen = false, sf_seen = false;
+            bool ok = true, seen = false, sf_seen = false;
             const uint64_t desc_a = umma_desc_sw128(smem_u32(smem_a)), desc_b = umma_desc_sw128(smem_u32(smem_b));
             constexpr int U = C::kRound;
             const auto after = [](int st, int by) { return st + by >= S ? st + by - S : st + by; };
@@ -345,27 +354,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     if (sf_end) commit(&sf_empty[sg]);
                     if (last) commit(&tmem_full[acc]);
-                    any = true;
+                    mmas = true;
                     seen = look;
                     phase = next_phase, stage = next;
                     if (sf_end) sf_seen = sf_look, sf_phase ^= sg_next == 0, sg = sg_next;
                 }
                 if (++acc == 2) acc = 0, acc_phase ^= 1u;
             }
-            if (!ok && any) {  // the MMAs issued so far end before TMEM is released
-                commit(&drain);
-                mbar_wait_drain(&drain, 0, 100000000ull);
-            }
         }
         __syncwarp();
     } else if (warp == 2) {
         int chunk = 0;
-        uint32_t phase = 0, issued = 0, issued_phase = 0;
+        uint32_t phase = 0;
         bool ok = true;
         for (int t = first; ok && t < total; t += step) {
             const Tile tile = tile_at<BN, PAIR, FOUR>(a, s_cut, s_tiles, t, m_blocks, rank);
             for (int b = 0; b < boxes; b += C::kChunkBoxes) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&chunk_empty[chunk], phase ^ 1u, abort_flag, a.status, kDevTimeoutProducer));
+                ok = __all_sync(0xffffffffu, wait(&chunk_empty[chunk], phase ^ 1u, kDevTimeoutProducer));
                 if (!ok) break;
                 if (elect_one()) {
                     uint8_t* dst = smem_s + chunk * C::kScaleBytes;
@@ -374,14 +379,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tma_load_2d(dst + kBlockM * C::kChunkBytes, &map_xs, &chunk_full[chunk], (box0 + b) * C::kBoxWords * 4, tile.row0);
                 }
                 __syncwarp();
-                issued |= 1u << chunk;
-                issued_phase = (issued_phase & ~(1u << chunk)) | (phase << chunk);
+                ++sent;
                 if (++chunk == C::kChunks) chunk = 0, phase ^= 1u;
             }
         }
-        if (!ok)
-            for (int i = 0; i < C::kChunks; ++i)
-                if (issued & (1u << i)) mbar_wait_drain(&chunk_full[i], (issued_phase >> i) & 1u, 100000000ull);
     } else if (warp >= 4 && warp < 8) {
         const uint32_t quad = static_cast<uint32_t>(warp & 3) * 32u << 16;
         constexpr int kXRows = (BN + 31) / 32;
@@ -391,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = first; ok && t < total; t += step) {
             for (int b = 0; b < boxes; b += C::kChunkBoxes) {
                 // Every lane waits for what it reads; a lane that gave up takes its warp along.
-                ok = mbar_wait(&chunk_full[chunk], chunk_phase, abort_flag, a.status, kDevTimeoutProducer);
+                ok = wait(&chunk_full[chunk], chunk_phase, kDevTimeoutProducer);
                 ok = __all_sync(0xffffffffu, ok && wait(&sf_empty[sg], phase ^ 1u, kDevTimeoutProducer));
                 if (!ok) break;
                 tc_fence_after();
@@ -496,9 +497,48 @@ __global__ void __launch_bounds__(kThreads, 1)
             cluster_sync();  // no CTA leaves while another reads its sums
         }
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if constexpr (PAIR) cluster_sync();  // neither CTA leaves while the other may signal it or use its memory
+    bool gave_up = s_abort != 0;
+    if constexpr (PAIR) {
+        if (gave_up && threadIdx.x == 0) st_cluster_u32(mapa_shared(smem_u32(&s_peer_gave_up), rank ^ 1), 1);
+        __syncwarp();
+        cluster_sync();  // neither CTA leaves while the other may signal it or use its memory
+        gave_up = gave_up || s_peer_gave_up != 0;
+    }
+    if (gave_up) {  // all warps, of both CTAs of a pair, have stopped
+        constexpr uint64_t limit = 100000000;  // 0.1 s, whatever the pipeline's own limit: copies in flight take microseconds
+        // The copies of the last round of a ring; those of earlier rounds have been consumed.
+        const auto land = [&](uint64_t* bars, uint32_t ring, uint32_t count) {
+            for (uint32_t j = count > ring ? count - ring : 0; j < count; ++j) mbar_wait_drain(&bars[j % ring], j / ring & 1u, limit);
+        };
+        uint32_t all = sent;
+        if constexpr (PAIR) {
+            if (rank == 1 && threadIdx.x == 0) st_cluster_u32(mapa_shared(smem_u32(&s_peer_sent), 0), sent);
+            __syncwarp();
+            cluster_sync();
+            // Stages that the second CTA sent and the first never announced: half of their bytes.
+            if (rank == 0 && threadIdx.x == 0) {
+                const uint32_t per_tile = (boxes + B - 1) / B;
+                for (uint32_t j = sent; j < s_peer_sent; ++j)
+                    mbar_arrive_expect_tx(&full[j % S], min(B, boxes - static_cast<int>(j % per_tile) * B) * box_bytes);
+            }
+            __syncwarp();
+            all = max(sent, s_peer_sent);
+        }
+        if (warp == 0 && rank == 0) land(full, S, all);
+        if (warp == 2) land(chunk_full, C::kChunks, sent);
+        if (mmas) {
+            if constexpr (PAIR) umma_commit_pair(mapa_shared(smem_u32(&drain), 0));
+            else umma_commit(&drain);
+            mbar_wait_drain(&drain, 0, limit);
+        }
+        __syncwarp();
+        tc_fence_before();
+        __syncthreads();
+        if constexpr (PAIR) cluster_sync();
+    }
     tc_fence_after();
     if (warp == 1) {
         if constexpr (PAIR) tmem_dealloc_pair(tmem, 512);
@@ -547,6 +587,10 @@ lm_status launch(const Matrix& w, const Matrix& x, int64_t k, Args a, int64_t ti
 }
 
 }  // namespace
+
+// Testing only (lm_ops_debug_set).
+std::atomic<uint64_t> g_wait_limit_ns{0};
+std::atomic<int> g_stall{0};
 
 cudaError_t ops_status(int** status) {
     void* p = nullptr;
@@ -612,6 +656,9 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
     a.split = split;
     a.out_dtype = out_dtype;
     a.out_pairs = out_stride % 2 == 0 && aligned(out, 4);
+    a.stall = g_stall.load(std::memory_order_relaxed);
+    a.wait_limit_ns = g_wait_limit_ns.load(std::memory_order_relaxed);
+    if (a.wait_limit_ns == 0) a.wait_limit_ns = kWaitLimitNs;
     if (const cudaError_t e = ops_status(&a.status); e != cudaSuccess) return context_free_finish(e);
     const Matrix mw{w, w_scales, groups * n}, mx{x, x_scales, rows};
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -625,6 +672,18 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
         else st = launch<128, false, FOUR>(mw, mx, k, a, tiles(m_blocks), s);
     });
     return st;
+}
+
+lm_status lm_ops_debug_set(int32_t knob, int64_t value) {
+    if (knob == LM_DEBUG_WAIT_LIMIT_NS && value >= 0 && value <= static_cast<int64_t>(kWaitLimitNs)) {
+        g_wait_limit_ns.store(static_cast<uint64_t>(value), std::memory_order_relaxed);
+        return LM_OK;
+    }
+    if (knob == LM_DEBUG_PRODUCT_STALL && value >= 0 && value <= LM_STALL_TMEM_EMPTY) {
+        g_stall.store(static_cast<int>(value), std::memory_order_relaxed);
+        return LM_OK;
+    }
+    return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_ops_debug_set: an unknown knob, a limit above 2 s or an unknown barrier");
 }
 
 lm_status lm_ops_sync(void* stream) {
