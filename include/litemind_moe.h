@@ -452,8 +452,10 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
                        const uint8_t* w_scales, int32_t groups, int64_t n, int64_t k, const int32_t* offsets, void* out,
                        int32_t out_dtype, int64_t out_stride, void* stream);
 /* Waits for the stream and reports a device-side timeout of the operators without a context
- * (lm_mx_matmul) on the current device since the last call, then clears it, as lm_moe_sync does for a context: LM_ERR_DEVICE_TIMEOUT, and the results of
- * the calls since then are invalid. */
+ * (lm_mx_matmul) on the current device since the last call for this stream, as lm_moe_sync does for
+ * a context: LM_ERR_DEVICE_TIMEOUT, and results since then are invalid.  The device does not know
+ * which stream a captured product ran on, so every stream hears of every timeout, once each, at its
+ * next call (a stream's first call: of those before it too).  Not for use in a capture. */
 lm_status lm_ops_sync(void* stream);
 /*
  * Testing hooks of that path, for the whole process; production code leaves them at 0.

@@ -283,8 +283,7 @@ const std::string& context_free_error();
 // The same message for an entry point without a context: a refused argument, or a launch's status.
 lm_status context_free_fail(lm_status status, const char* message) noexcept;
 lm_status context_free_finish(cudaError_t e) noexcept;
-// The current device's status word of the operators without a context (mx_matmul.cu), which
-// lm_ops_sync reads.
+// The current device's status word of the operators without a context (mx_matmul.cu).
 cudaError_t ops_status(int** status);
 
 // Raises `kernel`'s dynamic shared-memory limit to `bytes` on the current device.

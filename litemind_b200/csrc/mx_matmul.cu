@@ -29,6 +29,9 @@
 
 #include <algorithm>
 #include <atomic>
+#include <map>
+#include <mutex>
+#include <utility>
 
 namespace lm {
 namespace {
@@ -79,7 +82,8 @@ struct Args {
     int* status;
 };
 
-__device__ int g_status;  // the first device-side error since the last lm_ops_sync
+__device__ int g_status;       // the first device-side error of the process: which wait ran out
+__device__ unsigned g_stalls;  // CTAs that gave up so far; never cleared
 
 // Where group g's rows start (cut[g]) and its first column tile (tiles[g]); one warp.  Offsets are
 // clamped to the rows and to ascending order, so no value of theirs leads outside the matrices.
@@ -508,6 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         gave_up = gave_up || s_peer_gave_up != 0;
     }
     if (gave_up) {  // all warps, of both CTAs of a pair, have stopped
+        if (threadIdx.x == 0) atomicAdd(&g_stalls, 1u);
         constexpr uint64_t limit = 100000000;  // 0.1 s, whatever the pipeline's own limit: copies in flight take microseconds
         // The copies of the last round of a ring; those of earlier rounds have been consumed.
         const auto land = [&](uint64_t* bars, uint32_t ring, uint32_t count) {
@@ -584,6 +589,20 @@ lm_status launch(const Matrix& w, const Matrix& x, int64_t k, Args a, int64_t ti
     cfg.attrs = &cluster;
     cfg.numAttrs = ctas > 1 ? 1 : 0;
     return context_free_finish(cudaLaunchKernelEx(&cfg, kernel, map_w, map_x, map_ws, map_xs, a));
+}
+
+// Whether `count` CTAs that gave up on the device are news to the stream.  Nothing on the device is
+// cleared: each stream is told on its own, whichever asks first, since a captured product may have
+// run on any of them.  Streams are noted by the ids that CUDA never gives twice, once something stalled.
+bool news(int device, unsigned long long stream_id, unsigned count) {
+    static std::mutex lock;
+    static std::map<std::pair<int, unsigned long long>, unsigned> told;
+    const std::lock_guard<std::mutex> guard(lock);
+    const std::pair<int, unsigned long long> key{device, stream_id};
+    const auto it = told.find(key);
+    if (it == told.end() ? count == 0 : count == it->second) return false;
+    told[key] = count;
+    return count != 0;  // 0: the device was reset since
 }
 
 }  // namespace
@@ -688,15 +707,18 @@ lm_status lm_ops_debug_set(int32_t knob, int64_t value) {
 
 lm_status lm_ops_sync(void* stream) {
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    int code = 0;
-    cudaError_t e = cudaMemcpyFromSymbolAsync(&code, g_status, sizeof code, 0, cudaMemcpyDeviceToHost, s);
+    unsigned count = 0;
+    cudaError_t e = cudaMemcpyFromSymbolAsync(&count, g_stalls, sizeof count, 0, cudaMemcpyDeviceToHost, s);
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    unsigned long long id = 0;
+    int device = 0;
+    if (e == cudaSuccess) e = cudaStreamGetId(s, &id);
+    if (e == cudaSuccess) e = cudaGetDevice(&device);
     if (e != cudaSuccess) return context_free_finish(e);
-    if (code == 0) return LM_OK;
-    const int zero = 0;
-    e = cudaMemcpyToSymbolAsync(g_status, &zero, sizeof zero, 0, cudaMemcpyHostToDevice, s);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
-    if (e != cudaSuccess) return context_free_finish(e);
+    try {
+        if (!news(device, id, count)) return LM_OK;
+    } catch (...) {  // no memory or lock to note it: told again at the next call
+    }
     return context_free_fail(LM_ERR_DEVICE_TIMEOUT, "lm_ops_sync: a kernel gave up waiting; its results are invalid");
 }
 

@@ -78,3 +78,57 @@ def test_waits_that_run_out_anywhere(form, limit_ns):
     debug(0, 0)
     assert torch.equal(product(), want)
     ops.sync()
+
+
+def test_every_stream_is_told():
+    """One stream's sync does not take the failure away from another, whichever asks first."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = ops.mx_quantize(torch.randn(4, 256, generator=g, device="cuda"), "e4m3")
+    w = ops.mx_quantize(torch.randn(128, 256, generator=g, device="cuda"), "e2m1")
+    streams = [torch.cuda.Stream() for _ in range(3)]
+
+    def sync(stream):
+        with torch.cuda.stream(stream):
+            try:
+                ops.sync()
+            except _lib.LiteMindError as err:
+                assert err.status == _lib.LM_ERR_DEVICE_TIMEOUT
+                return True
+            return False
+
+    for s in streams:
+        sync(s)  # of stalls before this test
+    torch.cuda.synchronize()
+    for stalled in range(3):
+        debug(_lib.LM_STALL_TMEM_FULL, LIMIT_NS)
+        with torch.cuda.stream(streams[stalled]):
+            ops.mx_matmul(x, w)
+        debug(0, 0)
+        streams[stalled].synchronize()
+        assert [sync(s) for s in streams] == [True] * 3
+        assert [sync(s) for s in streams] == [False] * 3
+    sync(torch.cuda.current_stream())
+
+
+def test_replayed_stall_is_told_where_it_ran():
+    """A product captured on one stream and replayed on another: the stream that ran it hears of it."""
+    x = ops.mx_quantize(torch.randn(4, 256, device="cuda"), "e4m3")
+    w = ops.mx_quantize(torch.randn(128, 256, device="cuda"), "e2m1")
+    ops.mx_matmul(x, w)
+    torch.cuda.synchronize()
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    debug(_lib.LM_STALL_TMEM_FULL, LIMIT_NS)
+    with torch.cuda.graph(graph):
+        ops.mx_matmul(x, w)
+    debug(0, 0)
+    with torch.cuda.stream(other):
+        try:
+            ops.sync()  # of stalls before this test
+        except _lib.LiteMindError:
+            pass
+        graph.replay()
+        with pytest.raises(_lib.LiteMindError) as err:
+            ops.sync()
+    assert err.value.status == _lib.LM_ERR_DEVICE_TIMEOUT
+    with pytest.raises(_lib.LiteMindError):
+        ops.sync()
