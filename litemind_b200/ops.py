@@ -202,9 +202,11 @@ def mx_matmul(x: MxTensor, w: MxTensor, offsets=None, dtype=torch.bfloat16, out=
 
 
 def sync(device=None) -> None:
-    """lm_ops_sync: waits for the device's current stream and raises if a kernel gave up waiting."""
-    index = torch.cuda.current_device() if device is None else torch.device(device).index or 0
-    _call(load().lm_ops_sync, index)
+    """lm_ops_sync: waits for the device's current stream and raises if a kernel gave up waiting
+    (device: the current one by default, and for "cuda" without an index)."""
+    device = torch.device("cuda" if device is None else device)
+    _need(device.type == "cuda", "sync needs a CUDA device")
+    _call(load().lm_ops_sync, torch.cuda.current_device() if device.index is None else device.index)
 
 
 def add_rms_norm(hidden, delta, weight, eps: float, fmt: str = "e4m3", bf16: bool = False, out=None):
