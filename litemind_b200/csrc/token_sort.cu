@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     }
     int before = 0, total = here;
     if (ctas > 1) {
+        __syncwarp();  // the barrier's instructions are a converged warp's; experts may end inside one
         cluster_sync();
         if (e < experts) {
             total = 0;
@@ -94,6 +95,7 @@ __global__ void __launch_bounds__(kPlanThreads)
                 total += t;
             }
         }
+        __syncwarp();
         cluster_sync();  // a CTA may not end while another reads its totals
     }
     int incl = total;
