@@ -380,7 +380,8 @@ lm_status lm_moe_route_static(const float* router, const uint16_t* x, int32_t to
  *             drops the pair (an expert held elsewhere, a padded token)
  *   offsets   int32 [experts + 1]: expert e's rows are offsets[e] .. offsets[e + 1] - 1
  *   at        int32 [tokens, top_k]: the pair's row, -1 when dropped
- * top_k <= LM_SORT_MAX_TOP_K, experts <= 1024, tokens x top_k <= 2^31 - 1025.
+ * top_k <= LM_SORT_MAX_TOP_K, experts <= 1024, tokens x top_k <= 2^31 - 1025.  The three arrays
+ * must not overlap.
  */
 #define LM_SORT_MAX_TOP_K 64
 lm_status lm_moe_sort_plan(const int32_t* topk_idx, int64_t tokens, int32_t top_k, int32_t experts, int32_t* offsets,
@@ -388,7 +389,7 @@ lm_status lm_moe_sort_plan(const int32_t* topk_idx, int64_t tokens, int32_t top_
 /* rows[at[t, j]] = x[t] for every pair with 0 <= at < n_rows; other rows are left as they were.
  * `at` here and below is a plan's: no row stands in it twice.
  * Rows are plain bytes (row_bytes of them, strides in bytes), so values of any type, MX codes and
- * MX scales sort alike.  x and rows must not overlap. */
+ * MX scales sort alike.  rows must not overlap x or at (columns side by side in one buffer do not). */
 lm_status lm_moe_sort_rows(const void* x, int64_t x_stride, const int32_t* at, int64_t tokens, int32_t top_k,
                            int64_t row_bytes, void* rows, int64_t rows_stride, int64_t n_rows, void* stream);
 /* y[t] = sum over j of weights[t, j] * rows[at[t, j]] (weights NULL: 1), f32 sums in slot order,

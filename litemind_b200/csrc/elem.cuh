@@ -4,6 +4,7 @@
 
 #include <cstdint>
 #include <cstring>
+#include <numeric>
 #include <type_traits>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -96,10 +97,27 @@ struct Raw8 {
 
 // ── entry points ─────────────────────────────────────────────────────────
 inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
-// Whether two ranges of bytes share one; a null pointer is no range.
-inline bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x != 0 && y != 0 && x < y + static_cast<uintptr_t>(b_bytes) && y < x + static_cast<uintptr_t>(a_bytes);
+// Rows of `width` bytes, `stride` bytes apart; a null pointer has none.
+struct Span {
+    const void* p;
+    int64_t rows, stride, width;
+    Span(const void* start, int64_t bytes) : Span(start, 1, bytes, bytes) {}
+    Span(const void* start, int64_t n, int64_t step, int64_t bytes)
+        : p(start), rows(n == 1 || step == bytes ? 1 : n), stride(step), width(n == 1 || step == bytes ? n * bytes : bytes) {}
+};
+// Whether two of them share a byte.  Columns side by side in one buffer do not: rows are compared
+// modulo the strides' common step, which is exact for equal strides and for a single row, and for
+// others may call rows shared that only come near one another.
+inline bool overlap(const Span& a, const Span& b) {
+    if (a.p == nullptr || b.p == nullptr || a.rows <= 0 || b.rows <= 0 || a.width <= 0 || b.width <= 0) return false;
+    using Wide = unsigned __int128;  // strides are the caller's
+    const auto end = [](const Span& s) { return Wide(reinterpret_cast<uintptr_t>(s.p)) + Wide(s.rows - 1) * Wide(s.stride) + Wide(s.width); };
+    const Wide x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+    if (end(a) <= y || end(b) <= x) return false;
+    if (a.rows == 1 && b.rows == 1) return true;
+    const int64_t step = a.rows == 1 ? b.stride : b.rows == 1 ? a.stride : std::gcd(a.stride, b.stride);
+    const int64_t ahead = static_cast<int64_t>(y >= x ? (y - x) % Wide(step) : (Wide(step) - (x - y) % Wide(step)) % Wide(step));
+    return ahead < a.width || step - ahead < b.width;
 }
 inline int64_t elem_size(int32_t dtype) { return dtype == LM_DTYPE_F32 ? 4 : 2; }
 inline bool is_float_type(int32_t dtype) { return dtype == LM_DTYPE_F32 || dtype == LM_DTYPE_BF16 || dtype == LM_DTYPE_F16; }

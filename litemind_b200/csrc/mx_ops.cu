@@ -355,7 +355,7 @@ lm_status lm_gemm_add_rms_norm_mx(const void* hidden, int32_t dtype, const void*
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_gemm_add_rms_norm_mx: a null pointer, or data not 32-byte or scales not 16-byte aligned");
     // Each thread stores the sum over the values it loaded and nobody else's.
     const int64_t bytes = rows * count * elem_size(dtype), delta_bytes = rows * count * elem_size(delta_dtype);
-    if ((sum != hidden && overlap(sum, bytes, hidden, bytes)) || ((sum != delta || delta_dtype != dtype) && overlap(sum, bytes, delta, delta_bytes)))
+    if ((sum != hidden && overlap({sum, bytes}, {hidden, bytes})) || ((sum != delta || delta_dtype != dtype) && overlap({sum, bytes}, {delta, delta_bytes})))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_gemm_add_rms_norm_mx: sum overlaps a part of hidden or delta, or a delta of another type");
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     // Rows of a whole number of 16-byte words, all starting on one: eight columns a load.

@@ -363,9 +363,12 @@ lm_status lm_moe_sort_plan(const int32_t* topk_idx, int64_t tokens, int32_t top_
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_sort_plan: tokens x top_k beyond 2^31, top_k beyond 64 or experts beyond 1024");
     if (offsets == nullptr || !aligned(offsets, 4) || (tokens > 0 && (topk_idx == nullptr || at == nullptr || !aligned(topk_idx, 4) || !aligned(at, 4))))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_sort_plan: a null or misaligned pointer");
+    const int64_t pairs = tokens * top_k;
+    const Span idx(topk_idx, pairs * 4), places(at, pairs * 4), starts(offsets, (int64_t{experts} + 1) * 4);
+    if (overlap(idx, places) || overlap(idx, starts) || overlap(places, starts))
+        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_sort_plan: topk_idx, offsets and at overlap");
     // A cluster's launch and its two barriers cost 1.4 us more than one CTA, which takes 0.7 us for each
     // 1000 pairs (8000 pairs: one CTA 8.5 us, two 7.2, four 5.9, eight 5.2; 98304: 67 and 12.4).
-    const int64_t pairs = tokens * top_k;
     const int ctas = pairs <= 2048 ? 1 : kPlanCluster;
     const int smem = (kPlanWarps + 1) * experts * 4;
     if (smem > 40 * 1024)
@@ -393,6 +396,9 @@ lm_status lm_moe_sort_rows(const void* x, int64_t x_stride, const int32_t* at, i
     if (tokens == 0 || row_bytes == 0 || n_rows == 0) return LM_OK;
     if (x == nullptr || at == nullptr || rows == nullptr || !aligned(at, 4))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_sort_rows: a null or misaligned pointer");
+    const Span to(rows, touched(n_rows), rows_stride, row_bytes);
+    if (overlap(to, {x, tokens, x_stride, row_bytes}) || overlap(to, {at, tokens * top_k * 4}))
+        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_sort_rows: rows overlaps x or at");
     const uintptr_t all = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(rows) | static_cast<uintptr_t>(x_stride) |
                           static_cast<uintptr_t>(rows_stride) | static_cast<uintptr_t>(row_bytes);
     const auto go = [&](auto unit) {
@@ -419,7 +425,7 @@ lm_status lm_moe_unsort_rows(const void* rows, int32_t dtype, int64_t n_rows, co
     if ((rows == nullptr && n_rows > 0) || at == nullptr || y == nullptr || !aligned(rows, elem_size(dtype)) || !aligned(y, elem_size(y_dtype)) || !aligned(at, 4) ||
         !aligned(weights, 4))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows: a null or misaligned pointer");
-    if (overlap(rows, touched(n_rows) * cols * elem_size(dtype), y, tokens * cols * elem_size(y_dtype)))
+    if (overlap({rows, touched(n_rows) * cols * elem_size(dtype)}, {y, tokens * cols * elem_size(y_dtype)}))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows: y overlaps rows");
     const bool vec = cols % 8 == 0 && aligned(rows, 16) && aligned(y, 16);
     lm_status st = LM_OK;
@@ -453,7 +459,7 @@ lm_status lm_moe_unsort_rows_backward(const void* grad_y, const void* rows, int3
         !aligned(grad_weights, 4))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows_backward: a null or misaligned pointer");
     const int64_t row_bytes = cols * elem_size(dtype), rows_bytes = touched(n_rows) * row_bytes;
-    if (overlap(grad_y, tokens * row_bytes, grad_rows, rows_bytes) || (grad_rows != rows && overlap(rows, rows_bytes, grad_rows, rows_bytes)))
+    if (overlap({grad_y, tokens * row_bytes}, {grad_rows, rows_bytes}) || (grad_rows != rows && overlap({rows, rows_bytes}, {grad_rows, rows_bytes})))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows_backward: grad_rows overlaps grad_y or part of rows");
     const bool vec = cols % 8 == 0 && aligned(grad_y, 16) && aligned(rows, 16) && aligned(grad_rows, 16);
     with_dtype(dtype, [&](auto dt) {

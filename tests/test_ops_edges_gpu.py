@@ -7,7 +7,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
-from litemind_b200 import ops  # noqa: E402
+from litemind_b200 import _lib, ops  # noqa: E402
 from tests import mx_reference as ref  # noqa: E402
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -34,3 +34,30 @@ def test_sort_plan_over_a_cluster(experts):
     plan = ops.sort_plan(idx, experts)
     offsets, at = ref.sort_plan(idx.cpu(), experts)
     assert torch.equal(plan.offsets.cpu(), offsets) and torch.equal(plan.at.cpu(), at)
+
+
+def test_sort_rows_in_one_buffer():
+    """Columns side by side, and rows behind one another, of one buffer are not the same memory."""
+    plan = ops.sort_plan(torch.randint(0, 8, (40, 1), generator=gen(1), device="cuda", dtype=torch.int32), 8)
+    for cols, strided in ((20, True), (64, True), (100, False)):
+        buffer = normal(gen(cols), 80, 2 * cols)
+        x = buffer[:40, :cols] if strided else buffer.view(-1)[: 40 * cols].view(40, cols)
+        out = buffer[:40, cols:] if strided else buffer.view(-1)[40 * cols:80 * cols].view(40, cols)
+        want = ops.sort_rows(x.clone(), plan)
+        before = x.clone()
+        same_bits(ops.sort_rows(x, plan, out=out), want)
+        same_bits(x, before)
+        even, odd = buffer[:80:2, :cols], buffer[1:80:2, 5:cols + 5]
+        want = ops.sort_rows(even.clone(), plan)
+        same_bits(ops.sort_rows(even, plan, out=odd), want)
+
+
+def test_sort_rows_in_place_is_refused():
+    plan = ops.sort_plan(torch.randint(0, 8, (40, 1), generator=gen(1), device="cuda", dtype=torch.int32), 8)
+    buffer = normal(gen(2), 41, 64)
+    before = buffer.clone()
+    for x, out in ((buffer[:40], buffer[:40]), (buffer[:40], buffer[1:]), (buffer[:40, :32], buffer[:40, 31:63])):
+        with pytest.raises(_lib.LiteMindError, match="overlaps x or at"):
+            ops.sort_rows(x, plan, out=out)
+    torch.cuda.synchronize()
+    same_bits(buffer, before)
