@@ -431,10 +431,10 @@ int64_t lm_mx_scale_pitch(int64_t cols);
 /* values [rows, cols] of `dtype` (LM_DTYPE_F32, _BF16 or _F16), row_stride elements apart, to MX.
  * A block's scale byte is the biased f32 exponent of its largest magnitude less 2 (E2M1) or 8
  * (E4M3), at least 0; codes are rounded to nearest even and clamped to +-6 or +-448.  A block with
- * a NaN or an infinity gets scale byte 255 (NaN) and zero codes. */
+ * a NaN or an infinity gets scale byte 255 (NaN) and zero codes.  The three arrays must not overlap. */
 lm_status lm_mx_quantize(const void* values, int32_t dtype, int64_t rows, int64_t cols, int64_t row_stride, int32_t format,
                          uint8_t* data, uint8_t* scales, void* stream);
-/* The values that an MX matrix stands for, rounded to `dtype`. */
+/* The values that an MX matrix stands for, rounded to `dtype`; values must not overlap data or scales. */
 lm_status lm_mx_dequantize(const uint8_t* data, const uint8_t* scales, int32_t format, int64_t rows, int64_t cols,
                            void* values, int32_t dtype, int64_t row_stride, void* stream);
 /*
@@ -445,7 +445,7 @@ lm_status lm_mx_dequantize(const uint8_t* data, const uint8_t* scales, int32_t f
  *   offsets      device int32 [groups + 1]: group g's rows are offsets[g] .. offsets[g + 1] - 1
  *                (lm_moe_sort_plan's); NULL with groups = 1: all rows.  Values are clamped to
  *                [0, rows] and to ascending order; rows of no group are left as they were
- *   out          [rows, n], out_stride elements apart
+ *   out          [rows, n], out_stride elements apart; overlaps no input
  * rows <= 2^31 - 1025, k >= 1, groups <= LM_MX_MAX_GROUPS, groups * n <= 2^31 - 1025.  A NaN or infinity affects only its own row (x)
  * or its group's column (w).
  */

@@ -636,6 +636,11 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
     if (out == nullptr || !aligned(out, elem_size(out_dtype)) || !aligned(offsets, 4) || x == nullptr || x_scales == nullptr || w == nullptr || w_scales == nullptr ||
         !aligned(x, 32) || !aligned(x_scales, 16) || !aligned(w, 32) || !aligned(w_scales, 16))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_mx_matmul: a null pointer, or data not 32-byte or scales not 16-byte aligned");
+    const Span to(out, rows, out_stride * elem_size(out_dtype), n * elem_size(out_dtype));
+    const int64_t w_rows = groups * n, scale_pitch = mx_scale_pitch(k);
+    if (overlap(to, {x, rows * mx_data_pitch(x_format, k)}) || overlap(to, {x_scales, rows * scale_pitch}) || overlap(to, {w, w_rows * mx_data_pitch(LM_MX_E2M1, k)}) ||
+        overlap(to, {w_scales, w_rows * scale_pitch}) || overlap(to, {offsets, (int64_t{groups} + 1) * 4}))
+        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_mx_matmul: out overlaps an input");
     // The tile's width by the average rows of a group.  Groups are ragged, so a tile is wide enough for
     // most of them: a second tile reads the group's weights again.  (64 experts of 2816 x 2048, us with
     // 16, 32, 64 rows a tile and with a pair's 128, E4M3 rows: 4 a group 39, 41, 45, 49; 16: 51, 40, 44,

@@ -303,6 +303,10 @@ lm_status lm_mx_quantize(const void* values, int32_t dtype, int64_t rows, int64_
     if (rows == 0 || cols == 0) return LM_OK;
     if (values == nullptr || data == nullptr || scales == nullptr || !aligned(values, elem_size(dtype)) || !aligned(data, 32) || !aligned(scales, 16))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_mx_quantize: data must be 32-byte aligned and scales 16-byte aligned");
+    const Span from(values, rows, row_stride * elem_size(dtype), cols * elem_size(dtype)), codes(data, rows * mx_data_pitch(format, cols)),
+        bytes(scales, rows * mx_scale_pitch(cols));
+    if (overlap(codes, from) || overlap(bytes, from) || overlap(codes, bytes))
+        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_mx_quantize: values, data and scales overlap");
     const bool vec = aligned(values, 16) && row_stride * elem_size(dtype) % 16 == 0;
     const dim3 grid = grid_for(rows, mx_scale_pitch(cols) * kMxBlock);
     with_dtype(dtype, [&](auto dt) {
@@ -326,6 +330,9 @@ lm_status lm_mx_dequantize(const uint8_t* data, const uint8_t* scales, int32_t f
     if (rows == 0 || cols == 0) return LM_OK;
     if (values == nullptr || data == nullptr || scales == nullptr || !aligned(values, elem_size(dtype)) || !aligned(data, 32) || !aligned(scales, 16))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_mx_dequantize: data must be 32-byte aligned and scales 16-byte aligned");
+    const Span to(values, rows, row_stride * elem_size(dtype), cols * elem_size(dtype));
+    if (overlap(to, {data, rows * mx_data_pitch(format, cols)}) || overlap(to, {scales, rows * mx_scale_pitch(cols)}))
+        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_mx_dequantize: values overlaps data or scales");
     const bool vec = aligned(values, 16) && row_stride * elem_size(dtype) % 16 == 0;
     const dim3 grid = grid_for(rows, cols);
     with_dtype(dtype, [&](auto dt) {

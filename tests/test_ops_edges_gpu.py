@@ -61,3 +61,17 @@ def test_sort_rows_in_place_is_refused():
             ops.sort_rows(x, plan, out=out)
     torch.cuda.synchronize()
     same_bits(buffer, before)
+
+
+def test_mx_outputs_between_the_rows_of_inputs():
+    """A buffer's columns as input and its other columns as output: not the same memory."""
+    g = gen(3)
+    buffer = normal(g, 64, 200, dtype=BF16)
+    x = ops.mx_quantize(buffer[:, :96], "e4m3")
+    w = ops.mx_quantize(normal(g, 100, 96), "e2m1")
+    want = ops.mx_matmul(x, w)
+    same_bits(ops.mx_matmul(x, w, out=buffer[:, 96:196]), want)
+    same_bits(ops.mx_quantize(buffer[:, :96], "e4m3").data, x.data)
+    few = ops.MxTensor(w.data[:64].contiguous(), w.scales[:64].contiguous(), 96, "e2m1")
+    with pytest.raises(_lib.LiteMindError, match="overlaps an input"):
+        ops.mx_matmul(x, few, out=x.data.view(BF16))

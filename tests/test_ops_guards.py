@@ -64,3 +64,17 @@ def test_sort_overlaps(lib):
     refused(lib, "lm_moe_sort_rows", "overlaps", good, dict(rows=x), dict(rows=x + 127), dict(rows=x - 127), dict(rows=x + 4 * 256 + 127), dict(rows=x - 9 * 256),
             dict(rows=x + 2, rstride=2**40), dict(rows=x, rstride=128), dict(rows=x - 64, rstride=128, n=1), dict(rows=x + 1000, rstride=512), dict(rows=at), dict(rows=at + 39),
             dict(rows=at - 9 * 256 - 127), dict(rows=x, xstride=2**60, rstride=2**61))
+
+
+def test_mx_overlaps(lib):
+    a = places("values", "data", "scales")
+    v, d, s = a["values"], a["data"], a["scales"]
+    good = dict(values=v, dtype=_lib.LM_DTYPE_BF16, rows=4, cols=100, stride=200, fmt=_lib.LM_MX_E4M3, data=d, scales=s)
+    refused(lib, "lm_mx_quantize", "overlap", good, dict(data=v), dict(data=v + 1376), dict(data=v - 3 * 128), dict(data=v - 480), dict(scales=v), dict(scales=v + 3 * 400 + 192),
+            dict(scales=v - 48), dict(scales=d), dict(scales=d + 496), dict(data=s + 32), dict(data=s - 480))
+    good = dict(data=d, scales=s, fmt=_lib.LM_MX_E2M1, rows=4, cols=100, values=v, dtype=_lib.LM_DTYPE_F32, stride=100)
+    refused(lib, "lm_mx_dequantize", "overlaps", good, dict(values=d), dict(values=d + 252), dict(values=d - 1596), dict(values=s), dict(values=s + 60), dict(values=s - 1596))
+    a = places("x", "xs", "w", "ws", "offsets", "out")
+    good = dict(x=a["x"], xs=a["xs"], fmt=_lib.LM_MX_E4M3, rows=10, w=a["w"], ws=a["ws"], groups=4, n=64, k=100, offsets=a["offsets"], out=a["out"], dtype=_lib.LM_DTYPE_F32, stride=80)
+    size = dict(x=1280, xs=160, w=256 * 64, ws=256 * 16, offsets=20)
+    refused(lib, "lm_mx_matmul", "out overlaps an input", good, *[dict(out=a[i] + by) for i in size for by in (0, size[i] - 4, -9 * 320 - 252)])
