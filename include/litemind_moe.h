@@ -395,15 +395,15 @@ lm_status lm_moe_sort_rows(const void* x, int64_t x_stride, const int32_t* at, i
 /* y[t] = sum over j of weights[t, j] * rows[at[t, j]] (weights NULL: 1), f32 sums in slot order,
  * rounded once; a token without rows gets 0.  accumulate != 0 adds to y (before the rounding).
  * rows [n_rows, cols] of `dtype` (LM_DTYPE_F32, _BF16 or _F16); y [tokens, cols] of the same type
- * or f32, not overlapping rows.  Without weights this is also the gradient of lm_moe_sort_rows. */
+ * or f32, not overlapping rows, at or weights.  Without weights this is also the gradient of lm_moe_sort_rows. */
 lm_status lm_moe_unsort_rows(const void* rows, int32_t dtype, int64_t n_rows, const int32_t* at, const float* weights,
                              int64_t tokens, int32_t top_k, int64_t cols, void* y, int32_t y_dtype, int32_t accumulate,
                              void* stream);
 /* The gradient of lm_moe_unsort_rows with weights:
  *   grad_rows[at[t, j]] = weights[t, j] * grad_y[t]     (other rows are left as they were)
  *   grad_weights[t, j]  = <grad_y[t], rows[at[t, j]]>   (f32; 0 when dropped)
- * grad_y, rows and grad_rows of one type.  grad_rows may be rows itself, and overlaps neither it
- * otherwise nor grad_y. */
+ * grad_y, rows and grad_rows of one type.  grad_rows may be rows itself; otherwise the outputs
+ * overlap neither an input nor one another. */
 lm_status lm_moe_unsort_rows_backward(const void* grad_y, const void* rows, int32_t dtype, int64_t n_rows,
                                       const int32_t* at, const float* weights, int64_t tokens, int32_t top_k,
                                       int64_t cols, void* grad_rows, float* grad_weights, void* stream);
@@ -509,8 +509,8 @@ lm_status lm_gemm_rms_norm(float* values, const float* weight, int64_t rows, int
  * and norm, in f32, goes to an MX matrix [rows, count] (data, scales, format as above) and, with
  * out_bf16 not NULL, to bf16 [rows, count] (what lm_moe_route reads).  hidden and delta are f32 or
  * bf16 (LM_DTYPE_*), all rows contiguous; sum has hidden's type and may be hidden itself or delta
- * when their types agree, and overlaps neither otherwise; the other outputs overlap no input.  The
- * squares are summed in f64. */
+ * when their types agree, and overlaps neither otherwise; the other outputs overlap no input and no
+ * output.  The squares are summed in f64. */
 lm_status lm_gemm_add_rms_norm_mx(const void* hidden, int32_t dtype, const void* delta, int32_t delta_dtype,
                                   const float* weight, int64_t rows, int64_t count, float epsilon, void* sum,
                                   uint16_t* out_bf16, int32_t format, uint8_t* data, uint8_t* scales, void* stream);

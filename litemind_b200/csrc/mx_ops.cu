@@ -360,6 +360,13 @@ lm_status lm_gemm_add_rms_norm_mx(const void* hidden, int32_t dtype, const void*
         !aligned(sum, elem_size(dtype)) || (delta != nullptr && !aligned(delta, elem_size(delta_dtype))) || !aligned(weight, 4) ||
         !aligned(out_bf16, 2) || !aligned(data, 32) || !aligned(scales, 16))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_gemm_add_rms_norm_mx: a null pointer, or data not 32-byte or scales not 16-byte aligned");
+    const Span total(sum, rows * count * elem_size(dtype)), plain(out_bf16, rows * count * 2), codes(data, rows * mx_data_pitch(format, count)),
+        bytes_of_scales(scales, rows * mx_scale_pitch(count)), gain(weight, count * 4);
+    for (const Span* out : {&plain, &codes, &bytes_of_scales})
+        if (overlap(*out, {hidden, rows * count * elem_size(dtype)}) || overlap(*out, {delta, rows * count * elem_size(delta_dtype)}) || overlap(*out, gain) || overlap(*out, total))
+            return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_gemm_add_rms_norm_mx: out_bf16, data or scales overlaps an input or sum");
+    if (overlap(plain, codes) || overlap(plain, bytes_of_scales) || overlap(codes, bytes_of_scales) || overlap(total, gain))
+        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_gemm_add_rms_norm_mx: out_bf16, data and scales overlap, or sum overlaps weight");
     // Each thread stores the sum over the values it loaded and nobody else's.
     const int64_t bytes = rows * count * elem_size(dtype), delta_bytes = rows * count * elem_size(delta_dtype);
     if ((sum != hidden && overlap({sum, bytes}, {hidden, bytes})) || ((sum != delta || delta_dtype != dtype) && overlap({sum, bytes}, {delta, delta_bytes})))

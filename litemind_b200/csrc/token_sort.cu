@@ -425,8 +425,9 @@ lm_status lm_moe_unsort_rows(const void* rows, int32_t dtype, int64_t n_rows, co
     if ((rows == nullptr && n_rows > 0) || at == nullptr || y == nullptr || !aligned(rows, elem_size(dtype)) || !aligned(y, elem_size(y_dtype)) || !aligned(at, 4) ||
         !aligned(weights, 4))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows: a null or misaligned pointer");
-    if (overlap({rows, touched(n_rows) * cols * elem_size(dtype)}, {y, tokens * cols * elem_size(y_dtype)}))
-        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows: y overlaps rows");
+    const Span to(y, tokens * cols * elem_size(y_dtype));
+    if (overlap(to, {rows, touched(n_rows) * cols * elem_size(dtype)}) || overlap(to, {at, tokens * top_k * 4}) || overlap(to, {weights, tokens * top_k * 4}))
+        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows: y overlaps rows, at or weights");
     const bool vec = cols % 8 == 0 && aligned(rows, 16) && aligned(y, 16);
     lm_status st = LM_OK;
     with_dtype(dtype, [&](auto dt) {
@@ -461,6 +462,10 @@ lm_status lm_moe_unsort_rows_backward(const void* grad_y, const void* rows, int3
     const int64_t row_bytes = cols * elem_size(dtype), rows_bytes = touched(n_rows) * row_bytes;
     if (overlap({grad_y, tokens * row_bytes}, {grad_rows, rows_bytes}) || (grad_rows != rows && overlap({rows, rows_bytes}, {grad_rows, rows_bytes})))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows_backward: grad_rows overlaps grad_y or part of rows");
+    const Span to(grad_rows, rows_bytes), dots(grad_weights, tokens * top_k * 4), plan(at, tokens * top_k * 4), scale(weights, tokens * top_k * 4);
+    if (overlap(to, plan) || overlap(to, scale) || overlap(to, dots) || overlap(dots, plan) || overlap(dots, scale) || overlap(dots, {rows, rows_bytes}) ||
+        overlap(dots, {grad_y, tokens * row_bytes}))
+        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows_backward: grad_rows and grad_weights overlap, or overlap at, weights, rows or grad_y");
     const bool vec = cols % 8 == 0 && aligned(grad_y, 16) && aligned(rows, 16) && aligned(grad_rows, 16);
     with_dtype(dtype, [&](auto dt) {
         with_bool(vec, [&](auto v) {

@@ -78,3 +78,25 @@ def test_mx_overlaps(lib):
     good = dict(x=a["x"], xs=a["xs"], fmt=_lib.LM_MX_E4M3, rows=10, w=a["w"], ws=a["ws"], groups=4, n=64, k=100, offsets=a["offsets"], out=a["out"], dtype=_lib.LM_DTYPE_F32, stride=80)
     size = dict(x=1280, xs=160, w=256 * 64, ws=256 * 16, offsets=20)
     refused(lib, "lm_mx_matmul", "out overlaps an input", good, *[dict(out=a[i] + by) for i in size for by in (0, size[i] - 4, -9 * 320 - 252)])
+
+
+def test_norm_overlaps(lib):
+    a = places("hidden", "delta", "weight", "sum", "bf16", "data", "scales")
+    size = dict(hidden=4 * 64 * 4, delta=4 * 64 * 2, weight=256, sum=4 * 64 * 4, bf16=4 * 64 * 2, data=4 * 128, scales=4 * 16)
+    good = dict(hidden=a["hidden"], dtype=_lib.LM_DTYPE_F32, delta=a["delta"], ddtype=_lib.LM_DTYPE_BF16, weight=a["weight"], rows=4, count=64, eps=1e-6, sum=a["sum"],
+                bf16=a["bf16"], fmt=_lib.LM_MX_E4M3, data=a["data"], scales=a["scales"])
+    for out in ("bf16", "data", "scales"):
+        refused(lib, "lm_gemm_add_rms_norm_mx", "overlap", good, *[{out: a[i] + by} for i in a if i != out for by in (0, (size[i] - 1) // 32 * 32, -((size[out] - 1) // 32 * 32))])
+    refused(lib, "lm_gemm_add_rms_norm_mx", "overlap", good, *[dict(sum=a["weight"] + by) for by in (0, 252, -1020)])
+
+
+def test_way_back_overlaps(lib):
+    a = places("rows", "at", "weights", "y")
+    good = dict(rows=a["rows"], dtype=_lib.LM_DTYPE_BF16, n=6, at=a["at"], weights=a["weights"], tokens=3, k=2, cols=64, y=a["y"], ydtype=_lib.LM_DTYPE_F32, acc=0)
+    size = dict(rows=6 * 128, at=24, weights=24)
+    refused(lib, "lm_moe_unsort_rows", "y overlaps", good, *[dict(y=a[i] + by) for i in size for by in (0, size[i] - 4, 4 - 3 * 256)])
+    a = places("gy", "rows", "at", "weights", "gr", "gw")
+    good = dict(gy=a["gy"], rows=a["rows"], dtype=_lib.LM_DTYPE_F16, n=6, at=a["at"], weights=a["weights"], tokens=3, k=2, cols=64, gr=a["gr"], gw=a["gw"])
+    size = dict(gy=3 * 128, rows=6 * 128, at=24, weights=24, gr=6 * 128)
+    refused(lib, "lm_moe_unsort_rows_backward", "overlap", good, *[dict(gw=a[i] + by) for i in size for by in (0, size[i] - 4, -20)],
+            *[dict(gr=a[i] + by) for i in ("gy", "at", "weights", "gw") for by in (0, 20, 4 - 6 * 128)], dict(gr=a["rows"] + 128), dict(gr=a["rows"] - 128))
