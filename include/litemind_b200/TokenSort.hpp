@@ -42,6 +42,13 @@ struct SortPlan {
                                            static_cast<int64_t>(tokens), top_k, static_cast<int64_t>(cols), grad_rows, grad_weights,
                                            stream);
     }
+    /** The same with grad_y in f32 whatever the type of the rows: the gradient of unsort with an f32 y. */
+    lm_status unsort_backward_f32(const float* grad_y, const void* rows, int32_t dtype, std::size_t n_rows, const float* weights,
+                                  std::size_t cols, void* grad_rows, float* grad_weights, void* stream = nullptr) const {
+        return lm_moe_unsort_rows_backward_f32(grad_y, rows, dtype, static_cast<int64_t>(n_rows), at, weights,
+                                               static_cast<int64_t>(tokens), top_k, static_cast<int64_t>(cols), grad_rows,
+                                               grad_weights, stream);
+    }
 };
 
 }  // namespace litemind::b200

@@ -407,6 +407,11 @@ lm_status lm_moe_unsort_rows(const void* rows, int32_t dtype, int64_t n_rows, co
 lm_status lm_moe_unsort_rows_backward(const void* grad_y, const void* rows, int32_t dtype, int64_t n_rows,
                                       const int32_t* at, const float* weights, int64_t tokens, int32_t top_k,
                                       int64_t cols, void* grad_rows, float* grad_weights, void* stream);
+/* The same with grad_y in f32 whatever the type of the rows: the gradient of lm_moe_unsort_rows with
+ * an f32 y. */
+lm_status lm_moe_unsort_rows_backward_f32(const float* grad_y, const void* rows, int32_t dtype, int64_t n_rows,
+                                          const int32_t* at, const float* weights, int64_t tokens, int32_t top_k,
+                                          int64_t cols, void* grad_rows, float* grad_weights, void* stream);
 
 /*
  * -- Microscaled (MX) matrices ----------------------------------------------------

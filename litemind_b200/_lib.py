@@ -101,6 +101,7 @@ SIGNATURES = {
     "lm_moe_sort_rows": (_i32, [_vp, _i64, _vp, _i64, _i32, _i64, _vp, _i64, _i64, _vp]),
     "lm_moe_unsort_rows": (_i32, [_vp, _i32, _i64, _vp, _vp, _i64, _i32, _i64, _vp, _i32, _i32, _vp]),
     "lm_moe_unsort_rows_backward": (_i32, [_vp, _vp, _i32, _i64, _vp, _vp, _i64, _i32, _i64, _vp, _vp, _vp]),
+    "lm_moe_unsort_rows_backward_f32": (_i32, [_vp, _vp, _i32, _i64, _vp, _vp, _i64, _i32, _i64, _vp, _vp, _vp]),
     "lm_mx_data_pitch": (_i64, [_i32, _i64]),
     "lm_mx_scale_pitch": (_i64, [_i64]),
     "lm_mx_quantize": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _vp, _vp, _vp]),

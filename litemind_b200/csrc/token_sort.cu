@@ -11,6 +11,7 @@
 #include "ptx.cuh"
 
 #include <algorithm>
+#include <cstdio>
 
 namespace lm {
 namespace {
@@ -262,13 +263,14 @@ __global__ void __launch_bounds__(kRowThreads, 3)
 }
 
 // grad_rows[at] = w grad_y, grad_weights = <grad_y, rows[at]> (0 for a dropped pair).  W warps of a
-// CTA take a token, its columns in turns, and add their dot products in order at the end.
-template <int DT, int V, int W>
+// CTA take a token, its columns in turns, and add their dot products in order at the end.  grad_y has
+// the rows' type or, as the output it belongs to, f32.
+template <int DT, int DG, int V, int W>
 __global__ void __launch_bounds__(kRowThreads, 3)
-    unsort_rows_backward_kernel(const typename Elem<DT>::T* __restrict__ grad_y, const typename Elem<DT>::T* rows, int64_t n_rows,
+    unsort_rows_backward_kernel(const typename Elem<DG>::T* __restrict__ grad_y, const typename Elem<DT>::T* rows, int64_t n_rows,
                                 const int32_t* __restrict__ at, const float* __restrict__ weights, int64_t tokens, int k, int64_t cols,
                                 typename Elem<DT>::T* grad_rows, float* __restrict__ grad_weights) {
-    constexpr int U = kStretches<DT, V>;
+    constexpr int U = kStretches<DG, V>;
     __shared__ float red[kRowWarps][LM_SORT_MAX_TOP_K];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * (kRowWarps / W) + warp / W;
@@ -286,7 +288,8 @@ __global__ void __launch_bounds__(kRowThreads, 3)
 #pragma unroll
                 for (int q = 0; q < kSlots; ++q) dot[q] = 0.0f;
                 for (int64_t c = (warp % W * 32 * U + lane) * V; c < cols; c += W * 32 * U * V) {
-                    Part<DT, V> g[U], v[kSlots][U];
+                    Part<DG, V> g[U];
+                    Part<DT, V> v[kSlots][U];
 #pragma unroll
                     for (int u = 0; u < U; ++u)
                         if (c + u * 32 * V < cols) g[u].load(grad_y + t * cols + c + u * 32 * V);
@@ -348,6 +351,57 @@ lm_status with_parts(int64_t tokens, int64_t parts, F&& f) {
 int64_t touched(int64_t n_rows) { return std::min<int64_t>(n_rows, INT32_MAX); }
 bool sizes_ok(int64_t tokens, int32_t k) {
     return tokens >= 0 && k > 0 && k <= LM_SORT_MAX_TOP_K && tokens <= (INT32_MAX - 1024) / k;  // 32-bit pair numbers, with room to step past the last
+}
+
+// The rows' gradient and the weights'; `who` names the entry in messages.
+lm_status unsort_backward(const char* who, const void* grad_y, int32_t grad_y_dtype, const void* rows, int32_t dtype, int64_t n_rows, const int32_t* at,
+                          const float* weights, int64_t tokens, int32_t top_k, int64_t cols, void* grad_rows, float* grad_weights, void* stream) {
+    const auto refuse = [&](const char* why) {
+        char message[192];
+        std::snprintf(message, sizeof message, "%s: %s", who, why);
+        return context_free_fail(LM_ERR_INVALID_ARGUMENT, message);
+    };
+    if (!is_float_type(dtype)) return refuse("tensors are f32, bf16 or f16");
+    if (!sizes_ok(tokens, top_k) || n_rows < 0 || cols < 0 || cols > LM_MX_MAX_COLS)
+        return refuse("a size out of range");
+    if (tokens == 0) return LM_OK;
+    if (at == nullptr || weights == nullptr || grad_weights == nullptr || (cols > 0 && grad_y == nullptr) || (cols > 0 && n_rows > 0 && (rows == nullptr || grad_rows == nullptr)) ||
+        !aligned(grad_y, elem_size(grad_y_dtype)) || !aligned(rows, elem_size(dtype)) || !aligned(grad_rows, elem_size(dtype)) || !aligned(at, 4) || !aligned(weights, 4) ||
+        !aligned(grad_weights, 4))
+        return refuse("a null or misaligned pointer");
+    const int64_t row_bytes = cols * elem_size(dtype), rows_bytes = touched(n_rows) * row_bytes, grad_y_bytes = tokens * cols * elem_size(grad_y_dtype);
+    if (overlap({grad_y, grad_y_bytes}, {grad_rows, rows_bytes}) || (grad_rows != rows && overlap({rows, rows_bytes}, {grad_rows, rows_bytes})))
+        return refuse("grad_rows overlaps grad_y or part of rows");
+    const Span to(grad_rows, rows_bytes), dots(grad_weights, tokens * top_k * 4), plan(at, tokens * top_k * 4), scale(weights, tokens * top_k * 4);
+    if (overlap(to, plan) || overlap(to, scale) || overlap(to, dots) || overlap(dots, plan) || overlap(dots, scale) || overlap(dots, {rows, rows_bytes}) ||
+        overlap(dots, {grad_y, grad_y_bytes}))
+        return refuse("grad_rows and grad_weights overlap, or overlap at, weights, rows or grad_y");
+    const bool vec = cols % 8 == 0 && aligned(grad_y, 16) && aligned(rows, 16) && aligned(grad_rows, 16);
+    with_dtype(dtype, [&](auto dt) {
+        with_bool(vec, [&](auto v) {
+            constexpr int DT = decltype(dt)::value, V = decltype(v)::value ? 8 : 1;
+            using T = typename Elem<DT>::T;
+            const auto go = [&](auto dg, auto warps) {
+                constexpr int DG = decltype(dg)::value, W = decltype(warps)::value, per = kRowWarps / W;
+                unsort_rows_backward_kernel<DT, DG, V, W><<<static_cast<unsigned>((tokens + per - 1) / per), kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+                    static_cast<const typename Elem<DG>::T*>(grad_y), static_cast<const T*>(rows), n_rows, at, weights, tokens, top_k, cols, static_cast<T*>(grad_rows),
+                    grad_weights);
+            };
+            // As many warps a token as its row has stretches for them (2048 bf16 columns, 16384 tokens:
+            // one warp 89 us, two 87, four 93, eight, half of them idle, 127; 1 token: 8.3, 5.6, 4.2).
+            const auto fit = [&](auto dg) {
+                constexpr int64_t piece = 32 * V * kStretches<decltype(dg)::value, V>;
+                const int64_t pieces = (cols + piece - 1) / piece;
+                if (pieces <= 1) go(dg, std::integral_constant<int, 1>{});
+                else if (pieces <= 2) go(dg, std::integral_constant<int, 2>{});
+                else if (pieces <= 4) go(dg, std::integral_constant<int, 4>{});
+                else go(dg, std::integral_constant<int, 8>{});
+            };
+            if (grad_y_dtype == LM_DTYPE_F32) fit(std::integral_constant<int, LM_DTYPE_F32>{});
+            else fit(dt);
+        });
+    });
+    return context_free_finish(cudaGetLastError());
 }
 
 }  // namespace
@@ -451,41 +505,12 @@ lm_status lm_moe_unsort_rows(const void* rows, int32_t dtype, int64_t n_rows, co
 
 lm_status lm_moe_unsort_rows_backward(const void* grad_y, const void* rows, int32_t dtype, int64_t n_rows, const int32_t* at, const float* weights,
                                       int64_t tokens, int32_t top_k, int64_t cols, void* grad_rows, float* grad_weights, void* stream) {
-    if (!is_float_type(dtype)) return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows_backward: tensors are f32, bf16 or f16");
-    if (!sizes_ok(tokens, top_k) || n_rows < 0 || cols < 0 || cols > LM_MX_MAX_COLS)
-        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows_backward: a size out of range");
-    if (tokens == 0) return LM_OK;
-    if (at == nullptr || weights == nullptr || grad_weights == nullptr || (cols > 0 && grad_y == nullptr) || (cols > 0 && n_rows > 0 && (rows == nullptr || grad_rows == nullptr)) ||
-        !aligned(grad_y, elem_size(dtype)) || !aligned(rows, elem_size(dtype)) || !aligned(grad_rows, elem_size(dtype)) || !aligned(at, 4) || !aligned(weights, 4) ||
-        !aligned(grad_weights, 4))
-        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows_backward: a null or misaligned pointer");
-    const int64_t row_bytes = cols * elem_size(dtype), rows_bytes = touched(n_rows) * row_bytes;
-    if (overlap({grad_y, tokens * row_bytes}, {grad_rows, rows_bytes}) || (grad_rows != rows && overlap({rows, rows_bytes}, {grad_rows, rows_bytes})))
-        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows_backward: grad_rows overlaps grad_y or part of rows");
-    const Span to(grad_rows, rows_bytes), dots(grad_weights, tokens * top_k * 4), plan(at, tokens * top_k * 4), scale(weights, tokens * top_k * 4);
-    if (overlap(to, plan) || overlap(to, scale) || overlap(to, dots) || overlap(dots, plan) || overlap(dots, scale) || overlap(dots, {rows, rows_bytes}) ||
-        overlap(dots, {grad_y, tokens * row_bytes}))
-        return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_moe_unsort_rows_backward: grad_rows and grad_weights overlap, or overlap at, weights, rows or grad_y");
-    const bool vec = cols % 8 == 0 && aligned(grad_y, 16) && aligned(rows, 16) && aligned(grad_rows, 16);
-    with_dtype(dtype, [&](auto dt) {
-        with_bool(vec, [&](auto v) {
-            constexpr int DT = decltype(dt)::value, V = decltype(v)::value ? 8 : 1;
-            using T = typename Elem<DT>::T;
-            const auto go = [&](auto warps) {
-                constexpr int W = decltype(warps)::value, per = kRowWarps / W;
-                unsort_rows_backward_kernel<DT, V, W><<<static_cast<unsigned>((tokens + per - 1) / per), kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-                    static_cast<const T*>(grad_y), static_cast<const T*>(rows), n_rows, at, weights, tokens, top_k, cols, static_cast<T*>(grad_rows), grad_weights);
-            };
-            // As many warps a token as its row has stretches for them (2048 bf16 columns, 16384 tokens:
-            // one warp 89 us, two 87, four 93, eight, half of them idle, 127; 1 token: 8.3, 5.6, 4.2).
-            const int64_t pieces = (cols + 32 * V * kStretches<DT, V> - 1) / (32 * V * kStretches<DT, V>);
-            if (pieces <= 1) go(std::integral_constant<int, 1>{});
-            else if (pieces <= 2) go(std::integral_constant<int, 2>{});
-            else if (pieces <= 4) go(std::integral_constant<int, 4>{});
-            else go(std::integral_constant<int, 8>{});
-        });
-    });
-    return context_free_finish(cudaGetLastError());
+    return unsort_backward("lm_moe_unsort_rows_backward", grad_y, dtype, rows, dtype, n_rows, at, weights, tokens, top_k, cols, grad_rows, grad_weights, stream);
+}
+
+lm_status lm_moe_unsort_rows_backward_f32(const float* grad_y, const void* rows, int32_t dtype, int64_t n_rows, const int32_t* at, const float* weights,
+                                          int64_t tokens, int32_t top_k, int64_t cols, void* grad_rows, float* grad_weights, void* stream) {
+    return unsort_backward("lm_moe_unsort_rows_backward_f32", grad_y, LM_DTYPE_F32, rows, dtype, n_rows, at, weights, tokens, top_k, cols, grad_rows, grad_weights, stream);
 }
 
 }  // extern "C"

@@ -318,13 +318,15 @@ def sort_rows_backward(grad_rows, plan: SortPlan, out=None, dtype=None):
 
 
 def unsort_rows_backward(grad_y, rows, plan: SortPlan, weights, out=None):
-    """lm_moe_unsort_rows_backward: (grad_rows, grad_weights) of unsort_rows with weights.
+    """lm_moe_unsort_rows_backward: (grad_rows, grad_weights) of unsort_rows with weights.  grad_y has
+    rows' type or is float32 (lm_moe_unsort_rows_backward_f32), as the result it belongs to.
     grad_rows goes to `out` (which may be rows itself); rows of no pair keep what it held
     (uninitialised without it)."""
     _need(rows.dim() == 2 and rows.is_contiguous(), "rows must be a contiguous matrix")
     code = _dtype(rows, "rows")
     (tokens, k), (n_rows, cols) = plan.at.shape, rows.shape
-    _full(grad_y, (tokens, cols), rows.dtype, "grad_y must be contiguous [tokens, cols] of rows' type")
+    wide = grad_y.dtype == torch.float32
+    _full(grad_y, (tokens, cols), torch.float32 if wide else rows.dtype, "grad_y must be contiguous [tokens, cols] of rows' type or float32")
     _full(weights, (tokens, k), torch.float32, "weights must be contiguous float32 [tokens, top_k]")
     index = _index(grad_y, rows, plan.at, weights, out)
     if out is None:
@@ -332,6 +334,6 @@ def unsort_rows_backward(grad_y, rows, plan: SortPlan, weights, out=None):
     else:
         _full(out, rows.shape, rows.dtype, "out must be contiguous, of rows' shape and type")
     grad_weights = torch.empty_like(weights)
-    _call(load().lm_moe_unsort_rows_backward, index, grad_y.data_ptr(), rows.data_ptr(), code, n_rows, plan.at.data_ptr(), weights.data_ptr(), tokens, k, cols,
+    _call(load().lm_moe_unsort_rows_backward_f32 if wide else load().lm_moe_unsort_rows_backward, index, grad_y.data_ptr(), rows.data_ptr(), code, n_rows, plan.at.data_ptr(), weights.data_ptr(), tokens, k, cols,
           out.data_ptr(), grad_weights.data_ptr())
     return out, grad_weights

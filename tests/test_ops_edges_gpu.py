@@ -75,3 +75,34 @@ def test_mx_outputs_between_the_rows_of_inputs():
     few = ops.MxTensor(w.data[:64].contiguous(), w.scales[:64].contiguous(), 96, "e2m1")
     with pytest.raises(_lib.LiteMindError, match="overlaps an input"):
         ops.mx_matmul(x, few, out=x.data.view(BF16))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("tokens,k,experts,dropped,cols", [(1, 1, 1, 0, 1), (5, 2, 3, 0.4, 71), (33, 6, 64, 0.3, 256), (300, 6, 16, 0, 2048), (64, 16, 40, 0.5, 1000),
+                                                            (20, 33, 8, 0.2, 96), (3, 8, 8, 0, 9000), (7, 3, 5, 1.1, 40)])
+def test_gradient_of_an_f32_result(tokens, k, experts, dropped, cols, dtype):
+    """grad_y in float32 with 16-bit rows: the products are rounded once, to the rows' type."""
+    g = gen(tokens + cols)
+    idx = torch.randint(0, experts, (tokens, k), generator=g, device="cuda", dtype=torch.int32)
+    idx[torch.rand(tokens, k, generator=g, device="cuda") < dropped] = -1
+    plan = ops.sort_plan(idx, experts)
+    at, live = plan.at.long(), plan.at >= 0
+    rows, gy = normal(g, tokens * k, cols, dtype=dtype), normal(g, tokens, cols)
+    weights = torch.rand(tokens, k, generator=g, device="cuda")
+    buffer = torch.full_like(rows, 7.0)
+    gr, gw = ops.unsort_rows_backward(gy, rows, plan, weights, out=buffer)
+    want = torch.full_like(rows, 7.0)
+    want[at[live]] = (gy.unsqueeze(1) * weights.unsqueeze(2)).to(dtype)[live]
+    same_bits(gr, want)
+    v = torch.where(live.unsqueeze(2), rows[at.clamp(min=0)].double(), torch.zeros(1, dtype=torch.float64, device="cuda"))
+    dots = v * gy.double().unsqueeze(1)
+    # cols products added in f32: each addition is off by half a step, 2^-24, of at most the sum of magnitudes
+    assert ((gw.double() - dots.sum(dim=2)).abs() <= cols * 2.0**-24 * dots.abs().sum(dim=2)).all() and (gw[~live] == 0).all()
+    clean = rows.clone()
+    gr2, gw2 = ops.unsort_rows_backward(gy, clean, plan, weights, out=clean)  # in place
+    same_bits(gr2[at[live]], gr[at[live]])
+    same_bits(gw2, gw)
+    odd = torch.empty(tokens * cols + 1, device="cuda")[1:].view(tokens, cols).copy_(gy)  # no 16-byte boundary
+    gr3, gw3 = ops.unsort_rows_backward(odd, rows, plan, weights, out=buffer.fill_(7.0))
+    same_bits(gr3, want)
+    assert ((gw3.double() - dots.sum(dim=2)).abs() <= cols * 2.0**-24 * dots.abs().sum(dim=2)).all()

@@ -100,3 +100,18 @@ def test_way_back_overlaps(lib):
     size = dict(gy=3 * 128, rows=6 * 128, at=24, weights=24, gr=6 * 128)
     refused(lib, "lm_moe_unsort_rows_backward", "overlap", good, *[dict(gw=a[i] + by) for i in size for by in (0, size[i] - 4, -20)],
             *[dict(gr=a[i] + by) for i in ("gy", "at", "weights", "gw") for by in (0, 20, 4 - 6 * 128)], dict(gr=a["rows"] + 128), dict(gr=a["rows"] - 128))
+
+
+def test_gradient_of_an_f32_result(lib):
+    """lm_moe_unsort_rows_backward_f32 refuses what its sibling refuses, with f32's alignment and size."""
+    a = places("gy", "rows", "at", "weights", "gr", "gw")
+    good = dict(gy=a["gy"], rows=a["rows"], dtype=_lib.LM_DTYPE_BF16, n=6, at=a["at"], weights=a["weights"], tokens=3, k=2, cols=64, gr=a["gr"], gw=a["gw"])
+    name = "lm_moe_unsort_rows_backward_f32"
+    refused(lib, name, name + ": tensors are", good, dict(dtype=0), dict(dtype=4))
+    refused(lib, name, name + ": a size", good, dict(n=-1), dict(tokens=-1), dict(tokens=2**30), dict(k=0), dict(k=65), dict(cols=-1), dict(cols=2**24 + 1))
+    refused(lib, name, name + ": a null or misaligned", good, dict(gy=None), dict(gy=a["gy"] + 2), dict(rows=None), dict(rows=a["rows"] + 1), dict(at=None), dict(at=a["at"] + 2),
+            dict(weights=None), dict(weights=a["weights"] + 2), dict(gr=None), dict(gr=a["gr"] + 1), dict(gw=None), dict(gw=a["gw"] + 2))
+    refused(lib, name, name + ": grad_rows overlaps", good, dict(gr=a["gy"]), dict(gr=a["gy"] + 3 * 256 - 2), dict(gr=a["rows"] + 128))
+    refused(lib, name, name + ": grad_rows and grad_weights", good, dict(gw=a["gy"] + 3 * 256 - 4), dict(gw=a["rows"]), dict(gw=a["weights"]), dict(gr=a["at"]))
+    order = list(good)
+    assert getattr(lib, name)(*[dict(good, tokens=0)[o] for o in order], None) == OK
