@@ -106,3 +106,36 @@ def test_gradient_of_an_f32_result(tokens, k, experts, dropped, cols, dtype):
     gr3, gw3 = ops.unsort_rows_backward(odd, rows, plan, weights, out=buffer.fill_(7.0))
     same_bits(gr3, want)
     assert ((gw3.double() - dots.sum(dim=2)).abs() <= cols * 2.0**-24 * dots.abs().sum(dim=2)).all()
+
+
+def test_documented_chain():
+    """The example of INTEGRATION.md as it stands there: it runs, and its gradients are the formulas'."""
+    import os
+
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")).read()
+    part = text[text.index("## Operators on their own"):]
+    part = part[: part.index("\n## ", 5)]
+    blocks = [b.split("```")[0] for b in part.split("```python\n")[1:]]
+    assert len(blocks) == 2
+    g = gen(17)
+    tokens, hidden, inter, experts, k = 29, 192, 96, 6, 2
+    idx = torch.randint(-1, experts, (tokens, k), generator=g, device="cuda", dtype=torch.int32)
+    names = dict(torch=torch, experts=experts, topk_idx=idx, topk_weights=torch.rand(tokens, k, generator=g, device="cuda"), hidden=normal(g, tokens, hidden),
+                 delta=normal(g, tokens, hidden), norm_weight=1 + 0.1 * normal(g, hidden), gate_up=0.1 * normal(g, experts, 2 * inter, hidden),
+                 down=0.1 * normal(g, experts, hidden, inter))
+    exec(blocks[0], names)
+    plan, y, delta = names["plan"], names["y"], names["delta"]
+    assert delta.dtype == F32 and delta.shape == (tokens, hidden) and y.shape == (tokens * k, hidden)
+    names.update(grad_delta=normal(g, tokens, hidden), grad_rows=normal(g, tokens * k, hidden))
+    exec(blocks[1], names)
+    at, live = plan.at.long().clamp(min=0), (plan.at >= 0).unsqueeze(2)
+    zero = torch.zeros(1, dtype=torch.float64, device="cuda")
+    dots = torch.where(live, y[at].double(), zero) * names["grad_delta"].double().unsqueeze(1)
+    assert ((names["grad_weights"].double() - dots.sum(dim=2)).abs() <= hidden * 2.0**-24 * dots.abs().sum(dim=2)).all()
+    want = names["grad_delta"].unsqueeze(1) * names["topk_weights"].unsqueeze(2)
+    same_bits(names["grad_y"][at[live[..., 0]]], want.to(BF16)[live[..., 0]])
+    terms = torch.where(live, names["grad_rows"][at].double(), zero)
+    assert ((names["grad_x"].double() - terms.sum(dim=1)).abs() <= k * 2.0**-24 * terms.abs().sum(dim=1)).all()
+    # and the result is the formula's on the stages before it
+    terms = torch.where(live, y[at].double(), zero) * names["topk_weights"].double().unsqueeze(2)
+    assert ((delta.double() - terms.sum(dim=1)).abs() <= (k + 1) * 2.0**-24 * terms.abs().sum(dim=1)).all()
