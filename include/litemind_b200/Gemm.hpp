@@ -51,12 +51,23 @@ inline lm_status rms_norm(float* values, const float* weight, std::size_t count,
     return lm_gemm_rms_norm(values, weight, 1, static_cast<int64_t>(count), epsilon, stream);
 }
 
-/** sum = hidden + delta and its RMS norm to an MX matrix (see Mx.hpp), in one pass; out_bf16 may be null. */
+/**
+ * sum = hidden + delta and its RMS norm to an MX matrix (see Mx.hpp), in one pass; delta and out_bf16
+ * may be null.  hidden (and sum) and delta are LM_DTYPE_F32 or LM_DTYPE_BF16.
+ */
+inline lm_status add_rms_norm_mx(const void* hidden, int32_t dtype, const void* delta, int32_t delta_dtype, const float* weight,
+                                 std::size_t rows, std::size_t count, float epsilon, void* sum, std::uint16_t* out_bf16,
+                                 int32_t format, std::uint8_t* data, std::uint8_t* scales, void* stream = nullptr) {
+    return lm_gemm_add_rms_norm_mx(hidden, dtype, delta, delta_dtype, weight, static_cast<int64_t>(rows), static_cast<int64_t>(count),
+                                   epsilon, sum, out_bf16, format, data, scales, stream);
+}
+
+/** The same with hidden, delta and sum in f32. */
 inline lm_status add_rms_norm_mx(const float* hidden, const float* delta, const float* weight, std::size_t rows,
                                  std::size_t count, float epsilon, float* sum, std::uint16_t* out_bf16, int32_t format,
                                  std::uint8_t* data, std::uint8_t* scales, void* stream = nullptr) {
-    return lm_gemm_add_rms_norm_mx(hidden, LM_DTYPE_F32, delta, LM_DTYPE_F32, weight, static_cast<int64_t>(rows),
-                                   static_cast<int64_t>(count), epsilon, sum, out_bf16, format, data, scales, stream);
+    return add_rms_norm_mx(hidden, LM_DTYPE_F32, delta, LM_DTYPE_F32, weight, rows, count, epsilon, sum, out_bf16, format, data,
+                           scales, stream);
 }
 
 /** In-place max-subtracted softmax. */

@@ -25,8 +25,13 @@ struct SortPlan {
     }
     /** rows[at[t, j]] = x[t], rows of row_bytes bytes each. */
     lm_status sort(const void* x, std::size_t row_bytes, void* rows, std::size_t n_rows, void* stream = nullptr) const {
-        const auto bytes = static_cast<int64_t>(row_bytes);
-        return lm_moe_sort_rows(x, bytes, at, static_cast<int64_t>(tokens), top_k, bytes, rows, bytes, static_cast<int64_t>(n_rows),
+        return sort(x, row_bytes, row_bytes, rows, row_bytes, n_rows, stream);
+    }
+    /** The same with rows of x and of the result x_stride and rows_stride bytes apart. */
+    lm_status sort(const void* x, std::size_t x_stride, std::size_t row_bytes, void* rows, std::size_t rows_stride, std::size_t n_rows,
+                   void* stream = nullptr) const {
+        return lm_moe_sort_rows(x, static_cast<int64_t>(x_stride), at, static_cast<int64_t>(tokens), top_k,
+                                static_cast<int64_t>(row_bytes), rows, static_cast<int64_t>(rows_stride), static_cast<int64_t>(n_rows),
                                 stream);
     }
     /** y[t] (+)= the sum over j of weights[t, j] * rows[at[t, j]]; without weights the gradient of sort. */

@@ -115,3 +115,12 @@ def test_gradient_of_an_f32_result(lib):
     refused(lib, name, name + ": grad_rows and grad_weights", good, dict(gw=a["gy"] + 3 * 256 - 4), dict(gw=a["rows"]), dict(gw=a["weights"]), dict(gr=a["at"]))
     order = list(good)
     assert getattr(lib, name)(*[dict(good, tokens=0)[o] for o in order], None) == OK
+
+
+def test_cpp_forms_take_every_type_and_stride(tmp_path):
+    import subprocess
+
+    from tests.test_cpp_mirror import _compile
+
+    res = subprocess.run([_compile("OpsFormsTest", tmp_path)], capture_output=True, text=True, timeout=60)
+    assert res.returncode == 0, res.stdout + res.stderr
