@@ -139,3 +139,29 @@ def test_documented_chain():
     # and the result is the formula's on the stages before it
     terms = torch.where(live, y[at].double(), zero) * names["topk_weights"].double().unsqueeze(2)
     assert ((delta.double() - terms.sum(dim=1)).abs() <= (k + 1) * 2.0**-24 * terms.abs().sum(dim=1)).all()
+
+
+def test_python_guards_behind_the_device_check():
+    """The guards that CPU tensors never reach, each by its own message."""
+    g = gen(5)
+    x, w = ops.mx_quantize(normal(g, 4, 64), "e4m3"), ops.mx_quantize(normal(g, 3, 5, 64), "e2m1")
+    offsets = torch.tensor([0, 1, 2, 4], device="cuda", dtype=torch.int32)
+    plan = ops.SortPlan(torch.zeros(9, device="cuda", dtype=torch.int32), torch.zeros(4, 1, device="cuda", dtype=torch.int32))
+    h, rows, weights, gain = normal(g, 4, 64), normal(g, 4, 64), torch.rand(4, 1, device="cuda"), torch.ones(64, device="cuda")
+    out = torch.zeros(4, 5, dtype=BF16, device="cuda")
+    cases = [(lambda: ops.mx_matmul(x, w), "several groups need offsets"), (lambda: ops.mx_matmul(x, w, offsets[:3]), "offsets must be int32"),
+             (lambda: ops.mx_matmul(x, w, offsets.long()), "offsets must be int32"), (lambda: ops.mx_matmul(x, w, torch.stack((offsets, offsets), 1)[:, 0]), "offsets must be int32"),
+             (lambda: ops.mx_matmul(x, w, offsets, out=out[:3]), "out has another shape or type"), (lambda: ops.mx_matmul(x, w, offsets, out=out.float()), "out has another shape or type"),
+             (lambda: ops.mx_matmul(x, w, offsets, out=out[:1].expand(4, 5)), "out must be a matrix"),
+             (lambda: ops.mx_matmul(x, w, offsets, dtype=torch.float64), "out must be float32, bfloat16"), (lambda: ops.mx_matmul(x, w, offsets.cpu()), "on one device"),
+             (lambda: ops.mx_dequantize(x, BF16, out=torch.zeros(4, 64, device="cuda")), "out has another shape or type"),
+             (lambda: ops.mx_dequantize(x, F32, out=torch.zeros(4, 65, device="cuda")[:, :64]), "not contiguous"), (lambda: ops.mx_dequantize(x, torch.float64), "out must be float32, bfloat16"),
+             (lambda: ops.add_rms_norm(h, None, gain, 1e-6, out=h[:3]), "out must be contiguous"), (lambda: ops.add_rms_norm(h, None, gain, 1e-6, out=h.to(BF16)), "out must be contiguous"),
+             (lambda: ops.add_rms_norm(h, None, gain.cpu(), 1e-6), "on one device"), (lambda: ops.unsort_rows_backward(h, rows, plan, weights, out=rows[:3]), "out must be contiguous"),
+             (lambda: ops.unsort_rows_backward(h, rows, plan, weights, out=rows.to(BF16)), "out must be contiguous"), (lambda: ops.sort_rows(h.cpu(), plan), "on a CUDA device"),
+             (lambda: ops.sort_rows(h, plan, out=rows.to(BF16)), "x's type and columns"), (lambda: ops.sort_rows(h, plan, out=rows[:, :63]), "x's type and columns"),
+             (lambda: ops.unsort_rows(rows, plan, weights.cpu()), "on one device")]
+    for n, (call, message) in enumerate(cases):
+        with pytest.raises(ValueError, match=message):
+            call()
+            pytest.fail(f"case {n} was not refused")

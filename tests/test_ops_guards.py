@@ -124,3 +124,88 @@ def test_cpp_forms_take_every_type_and_stride(tmp_path):
 
     res = subprocess.run([_compile("OpsFormsTest", tmp_path)], capture_output=True, text=True, timeout=60)
     assert res.returncode == 0, res.stdout + res.stderr
+
+
+def python_guards():
+    """(name, call, the guard's message): each call passes every other check that comes before a launch
+    except, on these CPU tensors, the one of the device."""
+    import torch
+
+    from litemind_b200 import ops
+
+    f32, bf16, i32 = torch.float32, torch.bfloat16, torch.int32
+    x, i, w = torch.zeros(4, 64), torch.zeros(4, 2, dtype=i32), torch.zeros(4, 2)
+    rows, gain = torch.zeros(8, 64), torch.ones(64)
+    plan = ops.SortPlan(torch.zeros(9, dtype=i32), i)
+    e4, e2 = ops.MxTensor.empty((4, 64), "e4m3", "cpu"), ops.MxTensor.empty((3, 5, 64), "e2m1", "cpu")
+    offsets = torch.zeros(4, dtype=i32)
+    data, scales = torch.zeros(4, 128, dtype=torch.uint8), torch.zeros(4, 16, dtype=torch.uint8)
+    return [
+        ("quantise type", lambda: ops.mx_quantize(x.double(), "e2m1"), "values must be float32"),
+        ("quantise format", lambda: ops.mx_quantize(x, "fp4"), "unknown MX format"),
+        ("quantise columns", lambda: ops.mx_quantize(x.t(), "e2m1"), "values must be a matrix with contiguous"),
+        ("quantise rows that repeat", lambda: ops.mx_quantize(x[:1].expand(4, 64), "e2m1"), "non-overlapping rows"),
+        ("quantise vector", lambda: ops.mx_quantize(x[0], "e2m1"), "values must be a matrix, or contiguous"),
+        ("quantise stack", lambda: ops.mx_quantize(torch.zeros(2, 64, 4).transpose(1, 2), "e2m1"), "contiguous with more dimensions"),
+        ("quantise out shape", lambda: ops.mx_quantize(x[:3], "e4m3", out=e4), "out has another shape or format"),
+        ("quantise out format", lambda: ops.mx_quantize(x, "e2m1", out=e4), "out has another shape or format"),
+        ("matrix format", lambda: ops.MxTensor(data, scales, 64, "e5m2"), "unknown MX format"),
+        ("matrix type", lambda: ops.MxTensor(data.int(), scales, 64, "e4m3"), "must be contiguous uint8"),
+        ("matrix strides", lambda: ops.MxTensor(data[:, ::2], scales, 64, "e2m1"), "must be contiguous uint8"),
+        ("matrix columns", lambda: ops.MxTensor(data, scales, 129, "e4m3"), "do not have the layout"),
+        ("matrix pitch", lambda: ops.MxTensor(data[:, :64].contiguous(), scales, 64, "e4m3"), "do not have the layout"),
+        ("matrix scales", lambda: ops.MxTensor(data, scales[:3], 64, "e4m3"), "do not have the layout"),
+        ("product columns", lambda: ops.mx_matmul(e4, ops.MxTensor.empty((3, 5, 63), "e2m1", "cpu"), offsets), "with the same k"),
+        ("product weights", lambda: ops.mx_matmul(e4, e4, None), "w 4-bit"),
+        ("product stack of x", lambda: ops.mx_matmul(e2, e2, offsets), "x must be"),
+        ("sort columns", lambda: ops.sort_rows(x.t(), plan), "x must be a matrix with contiguous"),
+        ("sort tokens", lambda: ops.sort_rows(x[:3], plan), "a row for each token"),
+        ("sort format", lambda: ops.sort_rows(e4, plan, out=ops.MxTensor.empty((8, 64), "e2m1", "cpu")), "format and columns"),
+        ("plan type", lambda: ops.sort_plan(i.long(), 8), "topk_idx must be contiguous int32"),
+        ("plan strides", lambda: ops.sort_plan(torch.zeros(2, 4, dtype=i32).t(), 8), "topk_idx must be contiguous int32"),
+        ("plan experts", lambda: ops.sort_plan(i, 0), "experts must be in"),
+        ("plan many experts", lambda: ops.sort_plan(i, 1025), "experts must be in"),
+        ("plan of other types", lambda: ops.SortPlan(torch.zeros(9), i), "offsets must be int32"),
+        ("plan of matrices", lambda: ops.SortPlan(i, i), "offsets must be int32"),
+        ("back rows", lambda: ops.unsort_rows(rows.t(), plan), "rows must be a contiguous matrix"),
+        ("back type", lambda: ops.unsort_rows(rows.double(), plan), "rows must be float32"),
+        ("back weights", lambda: ops.unsort_rows(rows, plan, torch.zeros(4, 3)), "weights must be contiguous float32"),
+        ("back weights type", lambda: ops.unsort_rows(rows, plan, w.half()), "weights must be contiguous float32"),
+        ("back to nothing", lambda: ops.unsort_rows(rows, plan, accumulate=True), "accumulate needs out"),
+        ("back to another type", lambda: ops.unsort_rows(rows, plan, dtype=torch.float16), "rows' type or float32"),
+        ("back to an out of another type", lambda: ops.unsort_rows(rows, plan, out=x.to(bf16)), "rows' type or float32"),
+        ("back to another shape", lambda: ops.unsort_rows(rows, plan, out=x[:3]), "out must be contiguous"),
+        ("gradient rows", lambda: ops.unsort_rows_backward(x, rows.t(), plan, w), "rows must be a contiguous matrix"),
+        ("gradient tokens", lambda: ops.unsort_rows_backward(x[:3], rows, plan, w), "grad_y must be contiguous"),
+        ("gradient type", lambda: ops.unsort_rows_backward(x.half(), rows, plan, w), "rows' type or float32"),
+        ("gradient other type", lambda: ops.unsort_rows_backward(x.half(), rows.to(bf16), plan, w), "rows' type or float32"),
+        ("gradient weights", lambda: ops.unsort_rows_backward(x, rows, plan, w[:, :1]), "weights must be contiguous float32"),
+        ("norm type", lambda: ops.add_rms_norm(x.half(), None, gain, 1e-6), "hidden must be contiguous"),
+        ("norm vector", lambda: ops.add_rms_norm(x[0], None, gain, 1e-6), "hidden must be contiguous"),
+        ("norm delta shape", lambda: ops.add_rms_norm(x, x[:2], gain, 1e-6), "delta must be contiguous"),
+        ("norm delta type", lambda: ops.add_rms_norm(x, x.half(), gain, 1e-6), "delta must be contiguous"),
+        ("norm weight", lambda: ops.add_rms_norm(x, None, gain[:63], 1e-6), "weight must be contiguous"),
+        ("norm weight type", lambda: ops.add_rms_norm(x, None, gain.to(bf16), 1e-6), "weight must be contiguous"),
+        ("norm format", lambda: ops.add_rms_norm(x, None, gain, 1e-6, fmt="e5m2"), "unknown MX format"),
+        # the device, one for each call
+        ("quantise on the CPU", lambda: ops.mx_quantize(x, "e2m1"), "on a CUDA device"),
+        ("dequantise on the CPU", lambda: ops.mx_dequantize(e4), "on a CUDA device"),
+        ("product on the CPU", lambda: ops.mx_matmul(e4, e2, offsets), "on a CUDA device"),
+        ("plan on the CPU", lambda: ops.sort_plan(i, 8), "on a CUDA device"),
+        ("sort on the CPU", lambda: ops.sort_rows(x, plan), "on a CUDA device"),
+        ("back on the CPU", lambda: ops.unsort_rows(rows, plan, w), "on a CUDA device"),
+        ("gradient on the CPU", lambda: ops.unsort_rows_backward(x, rows, plan, w), "on a CUDA device"),
+        ("norm on the CPU", lambda: ops.add_rms_norm(x, x, gain, 1e-6), "on a CUDA device"),
+    ]
+
+
+@pytest.mark.parametrize("case", range(54))
+def test_python_guards(case):
+    """Each guard by its own message: with the guard taken out another check would answer."""
+    pytest.importorskip("torch")
+    cases = python_guards()
+    assert len(cases) == 54
+    name, call, message = cases[case]
+    with pytest.raises(ValueError, match=message):
+        call()
+        pytest.fail(f"{name} was not refused")
