@@ -165,3 +165,78 @@ def test_python_guards_behind_the_device_check():
         with pytest.raises(ValueError, match=message):
             call()
             pytest.fail(f"case {n} was not refused")
+
+
+# ---------------------------------------------------------------- the residual norm
+
+# Every form of the kernel: one stretch of columns a thread, two (many bf16 rows), the sum read again
+# (rows wider than 8192), rows that start on 16-byte words and rows that do not.
+NORMS = [(3, 33), (5, 1000), (4, 2048), (3, 2049), (2, 6152), (1, 8200), (2, 40000), (15000, 500), (3700, 2048), (1250, 5001), (600, 16384), (400, 20001)]
+TYPES = [(F32, F32), (F32, BF16), (BF16, F32), (BF16, BF16), (BF16, None)]
+
+
+def grid_index(a, fmt):
+    """The index of the nearest of the format's magnitudes, ties to even, the largest for all beyond."""
+    grid = (ref.E2M1 if fmt == "e2m1" else ref.E4M3).to(a.device)
+    mid = (grid[1:] + grid[:-1]) / 2
+    lo = torch.searchsorted(mid, a.contiguous())
+    tie = (lo < mid.numel()) & (mid[lo.clamp(max=mid.numel() - 1)] == a)
+    return torch.where(tie & (lo % 2 == 1), lo + 1, lo)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("dtype,ddtype", TYPES)
+@pytest.mark.parametrize("rows,cols", NORMS)
+def test_norm_codes_are_the_nearest(rows, cols, dtype, ddtype, fmt):
+    """The codes are the f64 norm's own, and a neighbour's only where the norm is within its f32 error
+    of a midpoint: the inverse and two products are each off by half a step, 2^-24, 4 2^-24 in all with
+    their second-order terms.  The scale likewise, at the powers of two."""
+    g = gen(rows + cols)
+    hidden = (normal(g, rows, cols) * torch.exp2(3 * normal(g, rows, 1))).to(dtype)
+    delta = None if ddtype is None else normal(g, rows, cols, dtype=ddtype)
+    weight = 1 + 0.1 * normal(g, cols)
+    total, q, _ = ops.add_rms_norm(hidden, delta, weight, 1e-6, fmt=fmt)
+    x = total.double()
+    norm = x / torch.sqrt((x * x).mean(dim=1, keepdim=True) + 1e-6) * weight.double()
+    blocks, emax, by = -(-cols // 32), 2 if fmt == "e2m1" else 8, 4 * 2.0**-24
+    wide = torch.zeros(rows, blocks * 32, dtype=torch.float64, device="cuda")
+    wide[:, :cols] = norm
+    amax = wide.view(rows, blocks, 32).abs().amax(dim=2)
+    byte = q.scales[:, :blocks].long()
+
+    def scale_of(a):
+        return torch.where(a > 0, (torch.frexp(a).exponent.long() - 1 - emax + 127).clamp(min=0), torch.zeros_like(byte))
+
+    assert ((byte >= scale_of(amax * (1 - by))) & (byte <= scale_of(amax * (1 + by)))).all()
+    a = wide.abs() / ref.pow2(byte - 127).repeat_interleave(32, 1)
+    if fmt == "e4m3":
+        code = q.data[:, : blocks * 32].long()
+    else:
+        d = q.data[:, : blocks * 16].long()
+        code = torch.stack((d % 16, d // 16), dim=-1).flatten(-2)
+    sign_bit = 8 if fmt == "e2m1" else 128
+    assert ((code % sign_bit >= grid_index(a * (1 - by), fmt)) & (code % sign_bit <= grid_index(a * (1 + by), fmt))).all()
+    assert torch.equal(code >= sign_bit, torch.signbit(wide))
+    assert (q.scales[:, blocks:] == 0).all() and (q.data[:, blocks * (32 if fmt == "e4m3" else 16):] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,ddtype", TYPES)
+@pytest.mark.parametrize("rows,cols", NORMS)
+def test_norm_in_place(rows, cols, dtype, ddtype):
+    """The sum over hidden itself, and over delta where their types agree."""
+    g = gen(rows + cols)
+    hidden = normal(g, rows, cols, dtype=dtype)
+    delta = None if ddtype is None else normal(g, rows, cols, dtype=ddtype)
+    weight = 1 + 0.1 * normal(g, cols)
+    want = ops.add_rms_norm(hidden, delta, weight, 1e-6, bf16=True)
+    for over in ("hidden", "delta") if ddtype == dtype else ("hidden",):
+        h, d = hidden.clone(), None if delta is None else delta.clone()
+        total, q, plain = ops.add_rms_norm(h, d, weight, 1e-6, bf16=True, out=h if over == "hidden" else d)
+        assert total is (h if over == "hidden" else d)
+        same_bits(total, want[0])
+        same_bits(plain, want[2])
+        assert torch.equal(q.data, want[1].data) and torch.equal(q.scales, want[1].scales)
+        if d is not None and over == "hidden":
+            same_bits(d, delta)
+        if over == "delta":
+            same_bits(h, hidden)
