@@ -209,6 +209,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
         return mbar_wait(bar, parity, abort_flag, a.status, code, a.wait_limit_ns);
     };
+    const auto wait_both = [&](uint64_t* bar, uint32_t parity, int code) {  // on a barrier that both CTAs of a pair arrive on
+        return mbar_wait<PAIR>(bar, parity, abort_flag, a.status, code, a.wait_limit_ns);
+    };
     const auto commit = [&](uint64_t* bar) {
         if constexpr (PAIR) umma_commit_both(bar);
         else umma_commit(bar);
@@ -311,13 +314,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                 int width = BN;  // a pair's MMAs are no wider than the tile's rows need; one CTA's take 50 cycles at least
                 if constexpr (PAIR) width = mma_n<PAIR>(tile_at<BN, PAIR, FOUR>(a, s_cut, s_tiles, t, m_blocks, rank).rows);
                 const uint32_t shape = static_cast<uint32_t>(width >> 3) << 17;
-                ok = wait(&tmem_empty[acc], acc_phase ^ 1u, kDevTimeoutMma);
+                ok = wait_both(&tmem_empty[acc], acc_phase ^ 1u, kDevTimeoutMma);
                 const uint32_t d = tmem + acc * BN;
                 for (int b = 0; ok && b < boxes; b += U * B) {
                     const int stages = min(U, (boxes - b + B - 1) / B);
                     const bool sf_begin = b % C::kChunkBoxes == 0;
                     if ((sf_begin && !sf_seen) || !seen) {
-                        ok = !sf_begin || sf_seen || wait(&sf_full[sg], sf_phase, kDevTimeoutMma);
+                        ok = !sf_begin || sf_seen || wait_both(&sf_full[sg], sf_phase, kDevTimeoutMma);
 #pragma unroll
                         for (int u = 0; u < U; ++u)
                             if (u < stages) ok = ok && wait(&full[after(stage, u)], phase ^ (stage + u >= S), kDevTimeoutMma);
@@ -333,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     bool look = true;
 #pragma unroll
                     for (int u = 0; u < U; ++u) look = look && mbar_test(&full[after(next, u)], next_phase ^ (next + u >= S));
-                    const bool sf_look = sf_end && mbar_test(&sf_full[sg_next], sf_phase ^ (sg_next == 0));
+                    const bool sf_look = sf_end && mbar_test<PAIR>(&sf_full[sg_next], sf_phase ^ (sg_next == 0));
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
                         if (u >= stages) break;
