@@ -34,7 +34,8 @@ and the line reports the worst over ranks.
   roofline   the dominant kernel: algorithmic bytes per launch / its mean device
              time, against MEASURED_PEAKS.json
   cpu_baseline  the reference's own CPU code (oracle/_ref, built from the
-             reference's sources) on the host's cores, rank 0, N=1 only
+             reference's sources) on the host's cores, rank 0, N=1 only; null
+             where that library is not built
 --impl reference: the reference CPU path alone (rank 0), same metric and workload,
 a bounded sample of the batch per step.
 
@@ -229,6 +230,14 @@ def gate_up_bytes(shape, touched_experts: int, T: int) -> int:
 
 # ── reference CPU path ────────────────────────────────────────────────────
 
+def reference_missing() -> str | None:
+    """Why the reference's own CPU code cannot run here, or None."""
+    from oracle import oracle as orc
+
+    return None if orc.reference_available() else \
+        "the reference's CPU library (oracle/_ref) is not built: its sources are not on this machine"
+
+
 def cpu_reference_rate(weights, x_f32, seconds: float, min_reps: int = 1, max_reps: int = 1000, bias=None):
     """tokens/s of the reference's own MoE block (oracle/_ref) on all host threads."""
     from oracle.oracle import Reference, RouterConfig
@@ -256,6 +265,9 @@ def run_reference_arm(args, rank: int, world: int) -> None:
     if args.workload == "load":
         print(json.dumps({"impl": "reference", "unavailable": "the reference has no device loader (its WeightStore "
                                                               "maps shards and pages weights in on first touch)"}))
+        return
+    if missing := reference_missing():
+        print(json.dumps({"impl": "reference", "unavailable": missing}))
         return
     if args.workload == "ffn":
         g, u, d = dense_weights()
@@ -578,7 +590,7 @@ def run_ffn(args, rank: int, world: int, local_rank: int) -> int:
                      "traffic": None,
                      "share_of_step": {k: round(v[0] / total_prof, 4) for k, v in prof.items()} if total_prof else {}})
     cpu = None
-    if rank == 0 and not args.no_cpu_baseline:
+    if rank == 0 and not args.no_cpu_baseline and not reference_missing():
         xf = syn.bf16_to_f32(x_bits).reshape(T, H)
         cpu = cpu_dense_rate(g, u, d, xf, args.cpu_seconds)
     line = {
@@ -1096,7 +1108,7 @@ def run_layer(args, rank: int, world: int, local_rank: int) -> int:
         ep_base = measure_ep_base(layer, flush, args, torch)
 
     cpu = None
-    if rank == 0 and world == 1 and not args.no_cpu_baseline:
+    if rank == 0 and world == 1 and not args.no_cpu_baseline and not reference_missing():
         xf = syn.bf16_to_f32(x_bits).reshape(T, -1)
         # A bounded sample (at most 256 tokens) of the same batch, per-token rate.
         cpu = cpu_reference_rate(W, xf[:256], args.cpu_seconds, bias=bias_np)
