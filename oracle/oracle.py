@@ -318,6 +318,11 @@ def oracle() -> Oracle:
     return Oracle()
 
 
+def reference_sources() -> bool:
+    """Whether the reference's checkout is there to build from (an empty directory is none)."""
+    return os.path.isfile(os.path.join(REFERENCE_DIR, "src", "Gemm.cpp"))
+
+
 def reference_available() -> bool:
     return os.path.exists(REF_SO)
 

@@ -31,7 +31,7 @@ def reference_lib():
     from oracle import oracle as orc
 
     if not orc.reference_available():
-        if os.path.isdir(orc.REFERENCE_DIR):
+        if orc.reference_sources():
             orc.build()
         else:
             pytest.skip("reference build (oracle/_ref) is not available on this machine")
