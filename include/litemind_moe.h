@@ -515,7 +515,10 @@ lm_status lm_gemm_rms_norm(float* values, const float* weight, int64_t rows, int
  * out_bf16 not NULL, to bf16 [rows, count] (what lm_moe_route reads).  hidden and delta are f32 or
  * bf16 (LM_DTYPE_*), all rows contiguous; sum has hidden's type and may be hidden itself or delta
  * when their types agree, and overlaps neither otherwise; the other outputs overlap no input and no
- * output.  The squares are summed in f64. */
+ * output.  The squares are summed in f64.  sum is rounded to f32 and then to hidden's type where delta
+ * is f32 and hidden bf16.  rsqrt(...) is rounded to f32, so that with epsilon 0 a row whose root mean
+ * square is below 2^-127 (a row of zeros too) gives infinities and NaN, and one above 2^126 loses up to
+ * two bits of it. */
 lm_status lm_gemm_add_rms_norm_mx(const void* hidden, int32_t dtype, const void* delta, int32_t delta_dtype,
                                   const float* weight, int64_t rows, int64_t count, float epsilon, void* sum,
                                   uint16_t* out_bf16, int32_t format, uint8_t* data, uint8_t* scales, void* stream);

@@ -213,7 +213,8 @@ __device__ __forceinline__ void put_norm(float (&v)[8], float inverse, const flo
 }
 
 // The inverse root of the CTA's mean square: its first warp's work, 15% of the instructions of a row
-// of 2048 when every thread did it.
+// of 2048 when every thread did it.  Rounded to f32: it overflows below a root mean square of 2^-127, with
+// epsilon 0 only (a second factor for such rows cost the others 1% or more).
 template <int T>
 __device__ __forceinline__ float block_inverse(double s, double inv_cols, double eps) {
     __shared__ double red[32];

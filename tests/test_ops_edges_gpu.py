@@ -240,3 +240,28 @@ def test_norm_in_place(rows, cols, dtype, ddtype):
             same_bits(d, delta)
         if over == "delta":
             same_bits(h, hidden)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,cols", [(6, 33), (4, 2048), (2, 40000), (3700, 2048)])
+@pytest.mark.parametrize("size", [2.0**127, 2.0**126 * 1.2, 2.0**-120, 2.0**-125, 2.0**-126])
+def test_norm_at_the_ends_of_f32(size, rows, cols, dtype):
+    """Rows near f32's largest and least normal numbers, epsilon 0: the norm is of ordinary size all the same."""
+    g = gen(rows + cols)
+    hidden = ((0.5 + 0.5 * torch.rand(rows, cols, generator=g, device="cuda")) * torch.where(torch.rand(rows, cols, generator=g, device="cuda") < 0.5, -1.0, 1.0) * size).to(dtype)
+    weight = 1 + 0.1 * normal(g, cols)
+    _, _, plain = ops.add_rms_norm(hidden, None, weight, 0.0, bf16=True)
+    x = hidden.double()
+    norm = x / torch.sqrt((x * x).mean(dim=1, keepdim=True)) * weight.double()
+    # bf16's half step and, in f32, the inverse (half of 2^-149 of 2^-128 at worst) and two products
+    assert ((plain.double() - norm).abs() <= (2.0**-8 + 2.0**-22 + 2 * 2.0**-24) * norm.abs() * 1.001).all()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("power", [115, 100, -100, -118])
+def test_norm_codes_at_the_ends_of_f32(power, fmt):
+    """A power of two changes the norm of small whole numbers by nothing, as long as f32 holds the inverse."""
+    hidden = torch.randint(-15, 16, (3, 512), generator=gen(2), device="cuda").float()
+    weight = 1 + 0.1 * normal(gen(3), 512)
+    want, got = (ops.add_rms_norm(hidden * s, None, weight, 0.0, fmt=fmt)[1] for s in (1.0, 2.0**power))
+    assert torch.equal(got.data, want.data) and torch.equal(got.scales, want.scales)
