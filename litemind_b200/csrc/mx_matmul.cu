@@ -6,12 +6,12 @@
 // The weights are the MMA's M side, so that a few rows of X cost a narrow N instead of a padded M.
 // One persistent CTA an SM walks the tiles (group, BN rows of X, 128 rows of W); for many rows a
 // group, pairs of CTAs walk tiles of 256 rows of W by 128 of X together, each bringing its half of
-// both operands (L2 delivers about 57 bytes a cycle to an SM; at the full rate of the MMA a CTA of
-// its own asks for 92 and one of a pair for 62).
+// both operands (at the full rate of the MMA a CTA of its own asks the L2 for 92 bytes a cycle and one
+// of a pair for 62; a prompt's 24576 rows move 54 an SM and cycle, the dense shape below 42).
 // E4M3 rows of X take kind::mxf8f6f4, whose 4-bit operand is padded to a byte a code: W's codes
 // travel packed and the TMA spreads them in shared memory.  E2M1 rows take kind::mxf4 with both
-// operands packed, half the shared memory and half the MMAs (dense 4096 x 10944 x 2048: 51 us, 84
-// with E4M3 rows).
+// operands packed, half the shared memory and half the MMAs (dense 4096 x 10944 x 2048: 53 us, 84
+// to 91 with E4M3 rows, by the clock).
 // A CTA's warps:
 //   0      TMA producer: a ring of stages of two boxes of 128 bytes a row
 //   1      MMA issuer (of the pair's first CTA): four block-scaled MMAs a box
@@ -644,7 +644,9 @@ lm_status lm_mx_matmul(const uint8_t* x, const uint8_t* x_scales, int32_t x_form
     if (overlap(to, {x, rows * mx_data_pitch(x_format, k)}) || overlap(to, {x_scales, rows * scale_pitch}) || overlap(to, {w, w_rows * mx_data_pitch(LM_MX_E2M1, k)}) ||
         overlap(to, {w_scales, w_rows * scale_pitch}) || overlap(to, {offsets, (int64_t{groups} + 1) * 4}))
         return context_free_fail(LM_ERR_INVALID_ARGUMENT, "lm_mx_matmul: out overlaps an input");
-    // The tile's width by the average rows of a group.  Groups are ragged, so a tile is wide enough for
+    // The tile's width by the average rows of a group: of the buffer, since how many of them there are
+    // stands in the offsets on the device (768 rows of 64 groups in a buffer of 6144: 46 us, in one of 768
+    // 39; 96 of 8 groups in 768: 12.9, in 96 11.4).  Groups are ragged, so a tile is wide enough for
     // most of them: a second tile reads the group's weights again.  (64 experts of 2816 x 2048, us with
     // 16, 32, 64 rows a tile and with a pair's 128, E4M3 rows: 4 a group 39, 41, 45, 49; 16: 51, 40, 44,
     // 47; 40: 101, 64, 45, 49; 48: 64 rows 48, a pair 49; 59: 55 and 50.  Packed E2M1 rows: 4 a group 33,

@@ -392,7 +392,9 @@ lm_status lm_gemm_add_rms_norm_mx(const void* hidden, int32_t dtype, const void*
             // instructions bound, take two stretches a thread (us, two and one: 16384 x 2048 44 and 49, 4096 x
             // 8192 49 and 56, 4000 x 2048 12.8 and 13.3); fewer rows, where latency counts, and f32 rows,
             // which HBM bounds, take one (2000 x 2048 7.2 and 6.5, 8192 x 8192 f32 136 and 132).  Wider
-            // rows read their sum again (2048 x 16384: 63, held in registers 80).
+            // rows read their sum again (2048 x 16384: 63, held in registers 80; 20 to 32 bytes spilled).
+            // Below a class's top the CTA's last threads idle: rows of 2560 bf16 columns go at 68% of the
+            // rate of 2048, of 5120 at 86% of 4096's (f32: 89 and 88%).
             const bool many = rows * wide > int64_t(3) * 148 * 2048 * 8;
             const auto fit = [&](auto stretches) {
                 constexpr int C = decltype(stretches)::value;
