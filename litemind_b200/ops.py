@@ -325,7 +325,7 @@ def unsort_rows_backward(grad_y, rows, plan: SortPlan, weights, out=None):
     _need(rows.dim() == 2 and rows.is_contiguous(), "rows must be a contiguous matrix")
     code = _dtype(rows, "rows")
     (tokens, k), (n_rows, cols) = plan.at.shape, rows.shape
-    wide = grad_y.dtype == torch.float32
+    wide = grad_y.dtype == torch.float32 and rows.dtype != torch.float32
     _full(grad_y, (tokens, cols), torch.float32 if wide else rows.dtype, "grad_y must be contiguous [tokens, cols] of rows' type or float32")
     _full(weights, (tokens, k), torch.float32, "weights must be contiguous float32 [tokens, top_k]")
     index = _index(grad_y, rows, plan.at, weights, out)

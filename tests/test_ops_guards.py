@@ -209,3 +209,18 @@ def test_python_guards(case):
     with pytest.raises(ValueError, match=message):
         call()
         pytest.fail(f"{name} was not refused")
+
+
+def test_gradient_entry_by_types(monkeypatch):
+    """Only 16-bit rows with a float32 grad_y take the entry for it; messages name the entry that was called."""
+    torch = pytest.importorskip("torch")
+    from litemind_b200 import ops
+
+    called = []
+    monkeypatch.setattr(ops, "_index", lambda *tensors: 0)
+    monkeypatch.setattr(ops, "_call", lambda fn, *args: called.append(fn.__name__))
+    plan = ops.SortPlan(torch.zeros(9, dtype=torch.int32), torch.zeros(4, 2, dtype=torch.int32))
+    for rows_type, grad_type in ((torch.float32, torch.float32), (torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float32), (torch.float16, torch.float32)):
+        ops.unsort_rows_backward(torch.zeros(4, 8, dtype=grad_type), torch.zeros(8, 8, dtype=rows_type), plan, torch.zeros(4, 2))
+    name = "lm_moe_unsort_rows_backward"
+    assert called == [name, name, name + "_f32", name + "_f32"]
